@@ -325,6 +325,106 @@ int pe_kv_compact_batch(void* k_cache, void* v_cache, int batch, int64_t cache_s
                         int64_t cap, int hd, int dtype, const int64_t* seq_prefix, const int32_t* accept_out,
                         int max_seq_rows, void* stream);
 
+/* ------------------------------------------------------------ paged cache */
+/* A batch's K/V in pages, with a prefix that all sequences share. One layer of a
+ * pool is [num_pages][nkv][page_size][hd], page_size a power of two from 16 to
+ * 1024. A sequence's cached tokens (seq_len[b] of them, device int64) are the
+ * prefix_len shared ones, token i at row i % page_size of page
+ * prefix_table[i / page_size], followed by its own: token prefix_len + j at row
+ * j % page_size of page block_table[b][j / page_size] (device int32, rows
+ * ld_table entries apart, `cols` of them usable). Rows of sequence b in a call
+ * are [seq_row0[b], seq_row0[b + 1]) (device int32 [batch + 1], seq_row0[0] = 0);
+ * rows behind the last sequence belong to none and are left as they are. The
+ * reference keeps one contiguous cache per sequence (HF cache_utils.py:127-146)
+ * and has no counterpart of the paged calls; per sequence their results are
+ * those of the contiguous ones named below.
+ * Ids from device memory are checked before use: what is out of range sets a
+ * bit of `status` (PE_ERR_TREE: a row range; PE_ERR_CAPACITY: a length, or
+ * pages that are not there; PE_ERR_INDEX: a page, slot, path or sequence id)
+ * and is skipped. */
+/* Pages for the new rows, and their slots. Sequence b needs
+ * ceil((seq_len[b] - prefix_len + rows) / page_size) pages and holds held[b];
+ * the missing ones are taken from the end of free_pages[0 .. *free_top) in
+ * sequence order and written to its table. slots[r] (int64 [M]) = page *
+ * page_size + row of each new row, -1 for rows behind the last sequence and for
+ * rows that got no page. A sequence whose pages are not all there (the free list
+ * or its table's columns) gets none and sets PE_ERR_CAPACITY, as does every
+ * later one that needs a page. The new counts go to held_out [batch] and
+ * top_out [1]; where either is the input itself, `scratch`
+ * (pe_page_tables_scratch_bytes bytes) is needed, else it may be NULL, and
+ * held and free_top stay as they were. */
+int64_t pe_page_tables_scratch_bytes(int batch);
+int pe_page_tables(const int64_t* seq_len, const int32_t* seq_row0, int batch, int64_t M, int64_t prefix_len,
+                   int page_size, int32_t* block_table, int64_t ld_table, int64_t cols, int32_t* held,
+                   const int32_t* free_pages, int64_t n_free, int32_t* free_top, int32_t* held_out, int32_t* top_out,
+                   int32_t* scratch, int64_t* slots, int32_t* status, void* stream);
+/* The pages of the n listed sequences (device int32) back onto the free list;
+ * their table entries become -1 and held 0. n_free: the list's room. A sequence
+ * listed twice is returned once and sets PE_ERR_INDEX. */
+int pe_page_release(const int32_t* seqs, int n, int batch, int32_t* block_table, int64_t ld_table, int64_t cols,
+                    int32_t* held, int32_t* free_pages, int64_t n_free, int32_t* free_top, int32_t* status,
+                    void* stream);
+/* K/V rows to their slots, L layers: element (l, r, h, d) of k at l *
+ * k_strides[0] + r * k_strides[1] + h * k_strides[2] + d (elements; host arrays
+ * of three; v alike), pools [L][num_pages][nkv][page_size][hd]. Rows of a
+ * contiguous cache, or the k and v columns of a fused q/k/v block: what
+ * DynamicLayer.update's torch.cat (HF cache_utils.py:127-146) does to a
+ * contiguous cache. Rows of slot -1 are skipped; slots are distinct. */
+int pe_kv_write_paged(const void* k, const void* v, const int64_t* k_strides, const int64_t* v_strides, int L,
+                      int64_t M, int nkv, int hd, int dtype, void* k_pool, void* v_pool, int64_t num_pages,
+                      int page_size, const int64_t* slots, int32_t* status, void* stream);
+/* pe_kv_compact_batch through the block table: private rows p + path[i] of
+ * sequence b (p = seq_len[b] - prefix_len, the path from pe_accept_tree_batch's
+ * out with max_rows) move to p + i in every layer of the pools. */
+int pe_kv_compact_paged(void* k_pool, void* v_pool, int L, int nkv, int hd, int dtype, int64_t num_pages,
+                        int page_size, const int32_t* block_table, int64_t ld_table, int64_t cols, int batch,
+                        const int64_t* seq_len, int64_t prefix_len, const int32_t* accept_out, int max_rows,
+                        int32_t* status, void* stream);
+
+/* Attention of a batch's rows over the shared prefix and each sequence's own
+ * pages (its cached rows, then its rows of this call, which must have been
+ * written): per sequence what pe_tree_attention_batch computes, with the keys
+ * of the shared prefix read once for the rows of all sequences.
+ *   s = scale * q . k; softcap > 0: s = softcap * tanh(s / softcap);
+ *   slopes: s -= slopes[head] * (position of the row - position of the key)
+ * A row sees every cached key, and of its own sequence's new rows those of its
+ * ancestor bits (PE_MASK_TREE) or those up to its own (PE_MASK_CAUSAL); with
+ * window > 0 only keys with position of the row - position of the key < window.
+ * A cached key's position is its index in the sequence (the prefix first), a
+ * new row's positions[r], or seq_len[b] + its row number with PE_MASK_CAUSAL. A
+ * row that sees no key gets zeros. fp32 softmax; 16-bit types round the
+ * unnormalised probabilities to the type for the PV product, as
+ * pe_tree_attention does. V of every key that some row of the same sequence
+ * sees must be finite. Any hd <= 256; bf16 / fp16 with hd 64 or 128 run on the
+ * matrix cores where q, the pools and out are 16-byte aligned with ld_q and
+ * ld_out multiples of 8. */
+typedef struct pe_paged_attention_args {
+  const void* q;       /* [M][nh][hd], rows ld_q elements apart */
+  const void* k_pool;  /* [num_pages][nkv][page_size][hd] */
+  const void* v_pool;
+  void* out;           /* [M][nh * hd], rows ld_out elements apart */
+  const int32_t* block_table;
+  const int32_t* prefix_table; /* [prefix_pages], NULL without a prefix */
+  const int32_t* seq_row0;
+  const int64_t* seq_len;
+  const uint64_t* bits;     /* [M][words] (PE_MASK_TREE) */
+  const int64_t* positions; /* [M]; needed with window or slopes */
+  const float* slopes;      /* [nh] or NULL */
+  void* workspace;          /* pe_attention_paged_workspace_bytes; no initial value */
+  int32_t* status;
+  int64_t workspace_bytes;
+  int64_t ld_q, ld_out, ld_table, table_cols, num_pages, prefix_pages, prefix_len;
+  int64_t max_len; /* bound of every seq_len: it and max_rows size the launch */
+  int64_t window;  /* 0: none */
+  int64_t M;
+  int32_t batch, max_rows, nh, nkv, hd, page_size, dtype, mask_mode, words;
+  float scale, softcap; /* softcap 0: none */
+  int32_t _reserved;
+} pe_paged_attention_args;
+int64_t pe_attention_paged_workspace_bytes(int64_t M, int batch, int nh, int nkv, int hd, int max_rows,
+                                           int64_t max_len, int64_t prefix_len, int dtype);
+int pe_tree_attention_paged(const pe_paged_attention_args* args, void* stream);
+
 /* ------------------------------------------------------------ tree proposal */
 #define PE_PROPOSE_MAX_DEPTH 16
 #define PE_PROPOSE_MAX_WIDTH 64

@@ -92,6 +92,18 @@ class PassArgs(C.Structure):
     ]
 
 
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [
+        ("q", vp), ("k_pool", vp), ("v_pool", vp), ("out", vp), ("block_table", vp), ("prefix_table", vp),
+        ("seq_row0", vp), ("seq_len", vp), ("bits", vp), ("positions", vp), ("slopes", vp), ("workspace", vp),
+        ("status", vp), ("workspace_bytes", i64), ("ld_q", i64), ("ld_out", i64), ("ld_table", i64),
+        ("table_cols", i64), ("num_pages", i64), ("prefix_pages", i64), ("prefix_len", i64), ("max_len", i64),
+        ("window", i64), ("M", i64), ("batch", i32), ("max_rows", i32), ("nh", i32), ("nkv", i32), ("hd", i32),
+        ("page_size", i32), ("dtype", i32), ("mask_mode", i32), ("words", i32), ("scale", f32), ("softcap", f32),
+        ("_reserved", i32),
+    ]
+
+
 # name -> (restype, argtypes); must list every function declared in include/pe_hip.h
 SIGNATURES: dict[str, tuple] = {
     "pe_status_string": (C.c_char_p, [C.c_int]),
@@ -149,6 +161,16 @@ SIGNATURES: dict[str, tuple] = {
     "pe_accept_tree_batch": (C.c_int, [vp, i64, vp, i64, i64, C.c_int, vp, C.c_int, C.c_int, vp, vp, vp, vp, vp]),
     "pe_kv_compact_batch": (C.c_int, [vp, vp, C.c_int, i64, C.c_int, C.c_int, i64, C.c_int, C.c_int, vp, vp,
                                       C.c_int, vp]),
+    "pe_page_tables_scratch_bytes": (i64, [C.c_int]),
+    "pe_page_tables": (C.c_int, [vp, vp, C.c_int, i64, i64, C.c_int, vp, i64, i64, vp, vp, i64, vp, vp, vp, vp, vp, vp,
+                                 vp]),
+    "pe_page_release": (C.c_int, [vp, C.c_int, C.c_int, vp, i64, i64, vp, vp, i64, vp, vp, vp]),
+    "pe_kv_write_paged": (C.c_int, [vp, vp, C.POINTER(i64), C.POINTER(i64), C.c_int, i64, C.c_int, C.c_int, C.c_int,
+                                    vp, vp, i64, C.c_int, vp, vp, vp]),
+    "pe_kv_compact_paged": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, i64, C.c_int, vp, i64, i64, C.c_int,
+                                      vp, i64, vp, C.c_int, vp, vp]),
+    "pe_attention_paged_workspace_bytes": (i64, [i64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, i64, i64, C.c_int]),
+    "pe_tree_attention_paged": (C.c_int, [C.POINTER(PagedAttentionArgs), vp]),
     "pe_loop_commit": (C.c_int, [vp, C.c_int, vp, vp, C.c_int, vp, i64, C.c_int, vp, vp, vp, i64, vp, vp, C.c_int,
                                  vp, vp, vp, vp]),
     "pe_loop_miss_commit": (C.c_int, [vp, C.c_int, vp, C.c_int, vp, C.c_int, vp, vp, i64, vp, vp, vp, vp, vp, vp]),

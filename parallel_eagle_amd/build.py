@@ -26,6 +26,7 @@ SOURCES = [
     "pe_attn.hip",
     "pe_tree.hip",
     "pe_loop.hip",
+    "pe_paged.hip",
     "pe_model.cpp",
 ]
 

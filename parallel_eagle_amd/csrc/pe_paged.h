@@ -1,0 +1,56 @@
+// What the paged attention's kernels share (not part of the C ABI).
+#pragma once
+
+#include "pe_common.h"
+#include "pe_internal.h"
+
+// A call's arguments as the kernels take them (by value).
+struct PagedAttn {
+  const void* q;  // [M][nh][hd], rows ld_q elements apart
+  const void* k_pool;  // [num_pages][nkv][1 << ps_log2][hd]
+  const void* v_pool;
+  void* out;  // [M][nh * hd], rows ld_out elements apart
+  const int32_t* block_table;  // [batch][cols], rows ld_table apart
+  const int32_t* prefix_table;
+  const int32_t* seq_row0;
+  const int64_t* seq_len;
+  const uint64_t* bits;  // [M][words], tree masks only
+  const int64_t* positions;  // [M], only where distances count
+  const float* slopes;  // [nh] or null
+  int32_t* status;
+  int64_t ld_q, ld_out, ld_table, cols, num_pages, prefix_len, max_len, window, M;
+  int batch, max_rows, nh, nkv, hd, ps_log2, mask_mode, words;
+  float scale, softcap;
+};
+
+// the running maximum of a row that has seen nothing (its sum is 0)
+constexpr float kPagedInitMax = -2.0e38f;
+
+// Sequence b's rows and private length. A sequence whose row range, length or
+// row count is outside what the call was sized for, or whose tokens do not fit
+// its table, is skipped by every workgroup alike (ok false, err the status bit;
+// err 0 for a sequence without rows).
+struct PagedSeq {
+  int row0, rows;
+  int64_t priv;
+  bool ok;
+  int err;
+};
+
+__device__ __forceinline__ PagedSeq paged_seq(const PagedAttn& a, int b) {
+  PagedSeq s;
+  s.row0 = a.seq_row0[b];
+  const int r1 = a.seq_row0[b + 1];
+  s.rows = r1 - s.row0;
+  s.priv = a.seq_len[b] - a.prefix_len;
+  s.err = 0;
+  if (s.row0 < 0 || s.rows < 0 || r1 > a.M || s.rows > a.max_rows)
+    s.err = PE_ERR_TREE;
+  else if (s.priv < 0 || s.priv > a.max_len - a.prefix_len || s.priv + s.rows > (a.cols << a.ps_log2))
+    s.err = PE_ERR_CAPACITY;
+  s.ok = s.err == 0 && s.rows > 0;
+  return s;
+}
+
+// pe_paged.hip: the call on the VALU (fp32, any head size up to 256).
+PE_INTERNAL int pe_internal_paged_valu(const PagedAttn& a, int dtype, hipStream_t st);
