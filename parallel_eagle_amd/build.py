@@ -27,6 +27,7 @@ SOURCES = [
     "pe_tree.hip",
     "pe_loop.hip",
     "pe_paged.hip",
+    "pe_paged_attn.hip",
     "pe_model.cpp",
 ]
 

@@ -54,3 +54,37 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttn& a, int b) {
 
 // pe_paged.hip: the call on the VALU (fp32, any head size up to 256).
 PE_INTERNAL int pe_internal_paged_valu(const PagedAttn& a, int dtype, hipStream_t st);
+
+// Partial results (O, running maximum in base 2, sum) of one KV head's rows,
+// kept in the order in which the matrix cores leave them: of every 32-row tile
+// the hd / 8 pieces [64 lanes][4 floats] (piece 4 h + c of lane ln + 32 g: dims
+// 32 h + 8 c + 4 g .. + 3 of row ln), so that writing and reading a tile are
+// whole KiB. Row r of a KV head is (token r / G, query head r % G), tokens
+// counted over the whole batch. Part p of KV head kvh: tiles from
+// (p * nkv + kvh) * tiles on.
+struct PagedParts {
+  float* o;
+  float* ml;  // [parts][nkv][tiles * 32][2]
+  int64_t tiles;
+  int pre_parts;  // parts of the prefix come first, then the private splits'
+};
+
+// The prefix's work: nkv * nblk row blocks of `block_rows` rows, each `steps`
+// key steps; workgroup w takes the units [w * per, (w + 1) * per) of that
+// sequence, so all workgroups do the same amount and a block is covered by a
+// few of them, its parts.
+struct PagedPrefix {
+  int64_t total, per, steps;
+  int nblk, block_rows;
+};
+
+__device__ __forceinline__ int64_t prefix_first_wg(const PagedPrefix& p, int64_t block) { return block * p.steps / p.per; }
+__device__ __forceinline__ int prefix_parts_of(const PagedPrefix& p, int64_t block) {
+  return (int)((block * p.steps + p.steps - 1) / p.per - prefix_first_wg(p, block)) + 1;
+}
+
+// pe_paged_attn.hip: the call on the matrix cores (bf16 / fp16, hd 64 or 128).
+PE_INTERNAL int64_t pe_internal_paged_mfma_bytes(int64_t M, int batch, int nh, int nkv, int hd, int max_rows,
+                                                 int64_t max_len, int64_t prefix_len);
+PE_INTERNAL int pe_internal_paged_mfma(const PagedAttn& a, int dtype, void* workspace, int64_t workspace_bytes,
+                                       hipStream_t st);

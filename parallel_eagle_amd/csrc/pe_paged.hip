@@ -609,16 +609,24 @@ extern "C" int pe_kv_compact_paged(void* k_pool, void* v_pool, int L, int nkv, i
 }
 
 // ------------------------------------------------------------------ attention
+static bool mfma_fits(int hd, int dtype) {
+  return (hd == 64 || hd == 128) && (dtype == PE_DTYPE_BF16 || dtype == PE_DTYPE_F16);
+}
+
 extern "C" int64_t pe_attention_paged_workspace_bytes(int64_t M, int batch, int nh, int nkv, int hd, int max_rows,
                                                       int64_t max_len, int64_t prefix_len, int dtype) {
-  return 0;
+  if (M <= 0 || batch <= 0 || nh <= 0 || nkv <= 0 || nh % nkv || max_rows <= 0 || prefix_len < 0 ||
+      max_len < prefix_len || !mfma_fits(hd, dtype))
+    return 0;
+  return pe_internal_paged_mfma_bytes(M, batch, nh, nkv, hd, max_rows, max_len, prefix_len);
 }
 
 extern "C" int pe_tree_attention_paged(const pe_paged_attention_args* p, void* stream) {
   if (!p) return PE_ERR_ARG;
   const int es = esize(p->dtype), psl = page_log2(p->page_size);
-  if (!p->q || !p->k_pool || !p->v_pool || !p->block_table || !p->seq_row0 || !p->seq_len || !p->out || !p->status ||
-      es == 0 || psl < 0)
+  const bool none = p->M == 0 || p->max_rows == 0;  // no rows: their buffers may be absent
+  if (!p->k_pool || !p->v_pool || !p->block_table || !p->seq_row0 || !p->seq_len || !p->status || es == 0 || psl < 0 ||
+      (!none && (!p->q || !p->out)))
     return PE_ERR_ARG;
   if (p->M < 0 || p->M >= (int64_t(1) << 31) || p->batch <= 0 || p->batch > 65535 || p->nh <= 0 || p->nkv <= 0 ||
       p->nh % p->nkv || p->hd <= 0 || p->hd > 256 || p->max_rows < 0 || p->max_rows > 65535 || p->prefix_len < 0 ||
@@ -629,13 +637,13 @@ extern "C" int pe_tree_attention_paged(const pe_paged_attention_args* p, void* s
     return PE_ERR_ARG;
   if (p->prefix_len > 0 && (!p->prefix_table || p->prefix_pages < ((p->prefix_len - 1) >> psl) + 1)) return PE_ERR_ARG;
   if (p->mask_mode == PE_MASK_TREE) {
-    if (!p->bits || p->words <= 0) return PE_ERR_ARG;
+    if ((!p->bits && !none) || p->words <= 0) return PE_ERR_ARG;
     if (p->words > PE_TREE_MAX_WORDS || p->max_rows > 64 * p->words) return PE_ERR_TREE;
   } else if (p->mask_mode != PE_MASK_CAUSAL) {
     return PE_ERR_ARG;
   }
-  if ((p->window > 0 || p->slopes) && !p->positions) return PE_ERR_ARG;
-  if (p->M == 0 || p->max_rows == 0) return PE_OK;
+  if ((p->window > 0 || p->slopes) && !p->positions && !none) return PE_ERR_ARG;
+  if (none) return PE_OK;
   PagedAttn a;
   a.q = p->q;
   a.k_pool = p->k_pool;
@@ -668,5 +676,9 @@ extern "C" int pe_tree_attention_paged(const pe_paged_attention_args* p, void* s
   a.words = p->words;
   a.scale = p->scale;
   a.softcap = p->softcap;
+  const bool aligned = (((uintptr_t)p->q | (uintptr_t)p->k_pool | (uintptr_t)p->v_pool | (uintptr_t)p->out) & 15) == 0 &&
+                       p->ld_q % 8 == 0 && p->ld_out % 8 == 0;
+  if (mfma_fits(p->hd, p->dtype) && aligned)
+    return pe_internal_paged_mfma(a, p->dtype, p->workspace, p->workspace_bytes, (hipStream_t)stream);
   return pe_internal_paged_valu(a, p->dtype, (hipStream_t)stream);
 }

@@ -1,0 +1,717 @@
+// Attention over a shared prefix and paged keys on the matrix cores (bf16 /
+// fp16, heads of 64 or 128).
+//
+//   out_r = sum_j 2^(s_rj - M) v_j / sum_j 2^(s_rj - M),  s in base 2
+//
+// splits over any partition of the keys into parts with their own maximum m_p,
+// sum l_p and weighted sum O_p, joined by weights 2^(m_p - M). The keys of the
+// prefix are the same for every row of the batch, so one KV head's rows of all
+// sequences (R = M G of them) meet them as one matrix product: each K / V byte
+// read serves a block of up to 256 rows, and the prefix is bound by the matrix
+// cores (and the exponentials beside them) where a per-sequence pass would read
+// it once per sequence. A sequence's own keys serve its own rows only.
+//
+// Two launches: the prefix's parts, then the sequences' own keys, whose
+// workgroups join the prefix's parts to theirs and write the output. A third
+// launch joins the parts where a sequence's own keys are split as well.
+//
+// Products as in the contiguous kernels: S^T = K Q^T (A = 32 keys, B = the
+// wave's 32 rows, held in registers), so that a lane owns one row and 16 of 32
+// keys; O^T += V^T P^T with P^T straight from the S^T registers, rounded to the
+// type (half a step per weight; its sum l is of the unrounded ones, so the
+// error is that of the weights alone), V^T by transposed LDS reads.
+
+#include "pe_paged.h"
+
+#include <algorithm>
+
+namespace {
+
+constexpr float kLog2e = 1.44269504088896341f;
+
+// Physical 16-byte chunk of logical chunk c of row `row` is c ^ swizzle(row).
+// 256-byte rows: (2i ^ 4i ^ j), i = row % 4, j = row / 4 % 4; 128-byte rows (two
+// to a bank line): the bits of row / 2 % 8 reversed. Both are bijections on 16
+// rows, so a K fragment's 16 rows fall on distinct banks, and move the upper
+// bits of the chunk among four neighbouring rows, so the transposed V reads do.
+template <int HD>
+__device__ __forceinline__ int swizzle(int row) {
+  if constexpr (HD == 128) {
+    const int i = row & 3, j = (row >> 2) & 3;
+    return ((i << 1) ^ (i << 2) ^ j) & 15;
+  } else {
+    const int i = (row >> 1) & 7;
+    return ((i & 1) << 2) | (i & 2) | (i >> 2);
+  }
+}
+template <int HD>
+__device__ __forceinline__ uint32_t lds_at(int row, int chunk) {
+  return (uint32_t)(row * (HD * 2) + ((chunk ^ swizzle<HD>(row)) << 4));
+}
+
+template <int DT>
+__device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+  if constexpr (DT == PE_DTYPE_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
+                                                  0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                   0, 0, 0);
+}
+
+// s_waitcnt with vmcnt = N, the other counters at their maxima
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+}
+
+// One list of pages as the key source of a KV head.
+struct Pages {
+  const int32_t* table;
+  int64_t lo, hi;  // keys read: [lo, hi), the others of a step as the nearest of them
+};
+
+// What a lane's row needs besides its Q.
+struct RowInfo {
+  int64_t node;   // causal: its token's index among the sequence's new rows; tree: unused
+  int rel;        // its position - the position of key 0 of the list (MOD)
+  float slope2;   // slope * log2 e (MOD)
+  uint64_t nb[PE_TREE_MAX_WORDS];
+};
+
+// The configuration of a workgroup: W waves = NT row tiles x NK key groups, each
+// wave SB 32-key blocks of a step, a ring of ST steps in LDS filled straight
+// from global memory (ST - 1 of them in flight while one is multiplied).
+template <int HD_, int W_, int NK_, int SB_, int ST_>
+struct Cfg {
+  static constexpr int HD = HD_, W = W_, NK = NK_, SB = SB_, ST = ST_;
+  static constexpr int NT = W / NK;
+  static constexpr int SK = 32 * NK * SB;            // keys of a step
+  static constexpr int kHalf = SK * HD * 2;          // bytes of a step's K (and of its V)
+  static constexpr int kStep = 2 * kHalf;
+  static constexpr int kChunks = 2 * SK / 16 / W;    // 16-key pieces of K or V a wave loads per step
+  static constexpr int kPerChunk = 16 * HD * 2 / 1024;  // load instructions of one
+  static constexpr int kLoads = kChunks * kPerChunk;
+  static constexpr int kMergeRow = HD / 2 + 4;       // floats per lane of a key group's hand-over (16-byte rows)
+  static constexpr int kMerge = NT * 64 * kMergeRow * 4;
+  static constexpr int kSmem = ST * kStep > kMerge || NK == 1 ? ST * kStep : kMerge;
+  static_assert(2 * SK / 16 % W == 0, "whole pieces per wave");
+};
+
+// One 64-bit-masked step's visibility, bit j: key kb0 + j. Tree rows see keys
+// below P and the nodes of their bits; causal rows those up to P + node.
+__device__ __forceinline__ uint64_t node_window(int64_t kb0, int64_t P, const uint64_t* nb) {
+  const int64_t off = kb0 - P;  // node index of key kb0
+  if (off <= -64) return ~0ull;
+  if (off < 0) {
+    const int j0 = (int)(-off);
+    return ((1ull << j0) - 1) | (nb[0] << j0);
+  }
+  if (off >= 64 * PE_TREE_MAX_WORDS) return 0ull;
+  const int wi = (int)(off >> 6), sh = (int)(off & 63);
+  const uint64_t a = wi == 0 ? nb[0] : wi == 1 ? nb[1] : wi == 2 ? nb[2] : nb[3];
+  const uint64_t b = wi == 0 ? nb[1] : wi == 1 ? nb[2] : wi == 2 ? nb[3] : 0ull;
+  return sh ? (a >> sh) | (b << (64 - sh)) : a;
+}
+__device__ __forceinline__ uint64_t below(int64_t n) {  // bits 0 .. n - 1
+  return n >= 64 ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1);
+}
+
+// The keys [s0 SK, s1 SK) of a list for the workgroup's row tiles: O^T, m, l of
+// the wave's tile over its key group, then joined over the key groups (valid in
+// key group 0). `P`: the list's cached keys, new rows follow (PRE: no new rows).
+// Every step's keys outside [pg.lo, pg.hi) are masked; `whole_to` is the first
+// key that some row of the tile may not see (tree or causal rows). npos (LDS):
+// positions of the new rows relative to key 0 (tree rows with MOD).
+template <int DT, typename C, bool MOD, bool PRE>
+__device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const Pages& pg, int kvh, int s0, int s1,
+                                       int64_t P, int new_rows, bool live, int64_t last_key, const RowInfo& ri,
+                                       const u32x4_t (&qf)[C::HD / 16], const int* npos, bool& bad,
+                                       f32x16_t (&o)[C::HD / 32], float& m, float& l) {
+  constexpr int HD = C::HD, SB = C::SB;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int ln = lane & 31, g = lane >> 5;
+  const int kg = wave / C::NT;
+  const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+  typedef const __attribute__((address_space(4))) int32_t* const_i32;  // read through the scalar cache
+  const const_i32 tab = (const_i32)(uintptr_t)uniform_ptr((const uint16_t*)pg.table);
+  const int psl = a.ps_log2;
+  const int64_t clo = pg.lo >> 4, chi = (pg.hi - 1) >> 4;
+  // the pages of this wave's pieces of a step, asked for a step ahead
+  int page[C::kChunks];
+  auto piece_of = [&](int step, int c) {
+    const int ch = (wave * C::kChunks + c) % (C::SK / 16);
+    const int64_t k = (int64_t)step * (C::SK / 16) + ch;
+    return k < clo ? clo : k > chi ? chi : k;
+  };
+  auto ask = [&](int step) {
+#pragma unroll
+    for (int c = 0; c < C::kChunks; ++c) page[c] = tab[(piece_of(step, c) << 4) >> psl];
+  };
+  auto issue = [&](int step) {
+    const uint32_t buf = lds_base + (step % C::ST) * C::kStep;
+#pragma unroll
+    for (int c = 0; c < C::kChunks; ++c) {
+      const int piece = wave * C::kChunks + c, ch = piece % (C::SK / 16);
+      const bool is_v = piece >= C::SK / 16;
+      const int64_t k16 = piece_of(step, c);
+      int pgid = page[c];
+      if (pgid < 0 || pgid >= a.num_pages) {
+        bad = true;
+        pgid = 0;
+      }
+      const int64_t row = ((((int64_t)pgid * a.nkv + kvh) << psl) + ((k16 << 4) & ((1 << psl) - 1)));
+      const uint16_t* src = uniform_ptr((const uint16_t*)(is_v ? a.v_pool : a.k_pool) + row * HD);
+      const uint32_t dst =
+          __builtin_amdgcn_readfirstlane(buf + (is_v ? C::kHalf : 0) + ch * 16 * HD * 2);
+      const int rlo = (int)max(pg.lo - (k16 << 4), (int64_t)0), rhi = (int)min(pg.hi - 1 - (k16 << 4), (int64_t)15);
+#pragma unroll
+      for (int i = 0; i < C::kPerChunk; ++i) {
+        constexpr int kLanes = HD / 8;  // lanes on a row
+        const int r = i * (64 / kLanes) + lane / kLanes;
+        const int rr = min(max(r, rlo), rhi);
+        lds_dma16(src, (uint32_t)(rr * (HD * 2) + (((lane % kLanes) ^ swizzle<HD>(r)) << 4)), dst + i * 1024);
+      }
+    }
+  };
+
+#pragma unroll
+  for (int h = 0; h < HD / 32; ++h)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[h][i] = 0.f;
+  m = kPagedInitMax;
+  l = 0.f;
+  const float scale2 = a.scale * kLog2e;
+  const bool tree = a.mask_mode == PE_MASK_TREE;
+  const float cap_in = MOD && a.softcap > 0.f ? 2.f * scale2 / a.softcap : 0.f, cap_out = a.softcap * kLog2e;
+
+  __syncthreads();  // the buffers' and hand-over's last readers are done
+  __builtin_amdgcn_s_waitcnt(0);  // Q has landed: no later wait of the compiler's covers the ring's loads
+  if (s0 < s1) ask(s0);
+#pragma unroll
+  for (int i = 0; i < C::ST - 1; ++i)
+    if (s0 + i < s1) {
+      issue(s0 + i);
+      if (s0 + i + 1 < s1) ask(s0 + i + 1);
+    }
+  for (int s = s0; s < s1; ++s) {
+    if (s1 - 1 - s >= C::ST - 2) wait_vm<(C::ST - 2) * C::kLoads>();
+    else wait_vm<0>();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // everyone's loads of step s have landed, and step s - 1's buffer is free
+    asm volatile("" ::: "memory");
+    if (s + C::ST - 1 < s1) {
+      issue(s + C::ST - 1);
+      if (s + C::ST < s1) ask(s + C::ST);
+    }
+    const int64_t kb0 = (int64_t)s * C::SK + kg * 32 * SB;
+    if (!live || kb0 > last_key) continue;  // wave-uniform: the tile sees no key of this step
+    const uint8_t* kbp = smem + (s % C::ST) * C::kStep + kg * 32 * SB * HD * 2;
+    const uint8_t* vbp = kbp + C::kHalf;
+    f32x16_t sc[SB];
+#pragma unroll
+    for (int sb = 0; sb < SB; ++sb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[sb][i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < HD / 16; ++j)
+#pragma unroll
+      for (int sb = 0; sb < SB; ++sb)
+        sc[sb] = mfma32<DT>(*(const u32x4_t*)(kbp + lds_at<HD>(32 * sb + ln, 2 * j + g)), qf[j], sc[sb]);
+    // sc[sb][i] is key kb0 + 32 sb + 8 (i / 4) + 4 g + i % 4 of the lane's row
+    bool node_step = false;
+    if constexpr (!PRE) node_step = kb0 + 32 * SB > P;
+    if constexpr (MOD) {
+      if (cap_in != 0.f) {
+        // cap tanh(s / cap) = cap (1 - 2 / (1 + e^(2 s / cap))): both ends exact
+#pragma unroll
+        for (int sb = 0; sb < SB; ++sb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float e = __builtin_amdgcn_exp2f(sc[sb][i] * cap_in);
+            sc[sb][i] = fmaf(-2.f * cap_out, __builtin_amdgcn_rcpf(1.f + e), cap_out);
+          }
+      } else {
+#pragma unroll
+        for (int sb = 0; sb < SB; ++sb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[sb][i] *= scale2;
+      }
+      const bool listed = node_step && tree;  // distances of new rows come from their positions
+      if (a.slopes || a.window > 0) {
+        const int d0 = ri.rel - (int)kb0 - 4 * g;
+        const int64_t w = a.window;
+#pragma unroll
+        for (int sb = 0; sb < SB; ++sb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int off = 32 * sb + 8 * (i >> 2) + (i & 3);
+            int dist = d0 - off;
+            if (listed) {
+              const int64_t u = kb0 + off + 4 * g - P;
+              const int np = npos[u < 0 ? 0 : u < new_rows ? (int)u : new_rows - 1];
+              dist = u < 0 ? dist : ri.rel - np;
+            }
+            sc[sb][i] = fmaf(-ri.slope2, (float)dist, sc[sb][i]);
+            if (w > 0) sc[sb][i] = (int64_t)dist < w ? sc[sb][i] : -INFINITY;
+          }
+      }
+    }
+    const bool edge = node_step || kb0 + 32 * SB > pg.hi || kb0 < pg.lo;
+    if (edge) {
+      uint64_t win = ~0ull;
+      if constexpr (!PRE) win = tree ? node_window(kb0, P, ri.nb) : below(P + ri.node + 1 - kb0);
+      win &= below(pg.hi - kb0) & ~below(pg.lo - kb0);
+      win >>= 4 * g;
+#pragma unroll
+      for (int sb = 0; sb < SB; ++sb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          sc[sb][i] = ((win >> (32 * sb + 8 * (i >> 2) + (i & 3))) & 1ull) ? sc[sb][i] : -INFINITY;
+    }
+    float bmax = -INFINITY;
+#pragma unroll
+    for (int sb = 0; sb < SB; ++sb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) bmax = fmaxf(bmax, sc[sb][i]);
+    bmax = fmaxf(bmax, __shfl_xor(bmax, 32, 64));
+    if constexpr (!MOD) bmax *= scale2;
+    const float mnew = fmaxf(m, bmax);
+    const float alpha = __builtin_amdgcn_exp2f(m - mnew);
+    float psum = 0.f;
+    uint32_t pb[SB][8];
+#pragma unroll
+    for (int sb = 0; sb < SB; ++sb)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(MOD ? sc[sb][i] - mnew : fmaf(sc[sb][i], scale2, -mnew));
+        const float p1 = __builtin_amdgcn_exp2f(MOD ? sc[sb][i + 1] - mnew : fmaf(sc[sb][i + 1], scale2, -mnew));
+        psum += p0 + p1;
+        pb[sb][i >> 1] = pack2_16<DT>(p0, p1);
+      }
+    psum += __shfl_xor(psum, 32, 64);
+    l = l * alpha + psum;
+    if (__builtin_amdgcn_ballot_w64(mnew != m) != 0ull) {
+#pragma unroll
+      for (int h = 0; h < HD / 32; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[h][i] *= alpha;
+    }
+    m = mnew;
+    // O^T += V^T P^T over the 16-key quarters of the step
+    const int qg = lane >> 4, jl = lane & 15;
+#pragma unroll
+    for (int c = 0; c < 2 * SB; ++c) {
+      const int sb = c >> 1, cq = c & 1;
+      const u32x4_t bp = {pb[sb][4 * cq], pb[sb][4 * cq + 1], pb[sb][4 * cq + 2], pb[sb][4 * cq + 3]};
+      const int kb = 16 * c + 4 * (qg >> 1) + (jl >> 2);
+#pragma unroll
+      for (int h = 0; h < HD / 32; ++h) {
+        const int db = 32 * h + 16 * (qg & 1) + 4 * (jl & 3);
+        typedef short s4v_t __attribute__((__vector_size__(4 * sizeof(short))));
+        typedef __attribute__((address_space(3))) s4v_t lds_s4v_t;
+        const uint2 lo = __builtin_bit_cast(
+            uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v_t*)(vbp + lds_at<HD>(kb, db >> 3) + (db & 7) * 2)));
+        const uint2 hi = __builtin_bit_cast(
+            uint2,
+            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v_t*)(vbp + lds_at<HD>(kb + 8, db >> 3) + (db & 7) * 2)));
+        const u32x4_t av = {lo.x, lo.y, hi.x, hi.y};
+        o[h] = mfma32<DT>(av, bp, o[h]);
+      }
+    }
+  }
+  if constexpr (C::NK > 1) {
+    // the key groups hand their (O, m, l) to group 0 in turn
+    const int tile = wave % C::NT;
+    float* mo = (float*)smem + (tile * 64 + lane) * C::kMergeRow;
+    for (int k = 1; k < C::NK; ++k) {
+      __syncthreads();
+      if (kg == k) {
+#pragma unroll
+        for (int h = 0; h < HD / 32; ++h)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            *(f32x4_t*)&mo[16 * h + 4 * c] = f32x4_t{o[h][4 * c], o[h][4 * c + 1], o[h][4 * c + 2], o[h][4 * c + 3]};
+        mo[HD / 2] = m;
+        mo[HD / 2 + 1] = l;
+      }
+      __syncthreads();
+      if (kg == 0) {
+        const float m1 = mo[HD / 2], l1 = mo[HD / 2 + 1];
+        const float mx = fmaxf(m, m1);
+        const float a0 = __builtin_amdgcn_exp2f(m - mx), a1 = __builtin_amdgcn_exp2f(m1 - mx);
+        l = a0 * l + a1 * l1;
+        m = mx;
+#pragma unroll
+        for (int h = 0; h < HD / 32; ++h)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const f32x4_t o1 = *(const f32x4_t*)&mo[16 * h + 4 * c];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[h][4 * c + i] = a0 * o[h][4 * c + i] + a1 * o1[i];
+          }
+      }
+    }
+  }
+}
+
+// Work item of workgroup `b` of `n`: neighbours in the sequence of items (which
+// share a KV head's keys) on one XCD (workgroup b starts on XCD b % 8).
+__device__ __forceinline__ int64_t xcd_item(int64_t b, int64_t n) { return n & 7 ? b : (b & 7) * (n >> 3) + (b >> 3); }
+
+template <int HD>
+__device__ __forceinline__ int64_t part_tile(const PagedParts& p, int nkv, int part, int kvh, int64_t tile) {
+  return (((int64_t)part * nkv + kvh) * p.tiles + tile) * (32 * HD);
+}
+
+template <int HD>
+__device__ __forceinline__ void store_part(const PagedParts& p, int nkv, int part, int kvh, int64_t row, int g,
+                                           const f32x16_t (&o)[HD / 32], float m, float l) {
+  float* dst = p.o + part_tile<HD>(p, nkv, part, kvh, row >> 5) + ((row & 31) + 32 * g) * 4;
+#pragma unroll
+  for (int h = 0; h < HD / 32; ++h)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      *(f32x4_t*)(dst + (4 * h + c) * 256) = f32x4_t{o[h][4 * c], o[h][4 * c + 1], o[h][4 * c + 2], o[h][4 * c + 3]};
+  if (g == 0) {
+    float2* ml = (float2*)p.ml + ((int64_t)part * nkv + kvh) * p.tiles * 32 + row;
+    *ml = make_float2(m, l);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The prefix
+// ---------------------------------------------------------------------------
+template <int DT, typename C, bool MOD>
+__global__ __launch_bounds__(64 * C::W, 2) void paged_prefix_kernel(PagedAttn a, PagedPrefix pp, PagedParts parts) {
+  constexpr int HD = C::HD;
+  __shared__ __align__(1024) uint8_t smem[C::kSmem];
+  __shared__ int s_lo[C::W];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int ln = lane & 31, g = lane >> 5, tile = wave % C::NT, kg = wave / C::NT;
+  const int G = a.nh / a.nkv;
+  const int64_t R = a.M * G;
+  const int64_t w = xcd_item(blockIdx.x, gridDim.x);
+  const int64_t uend = min(pp.total, (w + 1) * pp.per);
+  bool bad = false;
+  for (int64_t u = w * pp.per; u < uend;) {
+    const int64_t x = u / pp.steps;
+    const int s0 = (int)(u - x * pp.steps);
+    const int s1 = (int)min(pp.steps, s0 + (uend - u));
+    u += s1 - s0;
+    const int kvh = (int)(x / pp.nblk);
+    const int64_t row0 = (x - (int64_t)kvh * pp.nblk) * pp.block_rows + 32 * tile;
+    const bool live = row0 < R;
+    const int64_t row = min(row0 + ln, R - 1), tok = row / G;
+    const int hq = kvh * G + (int)(row - tok * G);
+    u32x4_t qf[HD / 16];
+    const uint16_t* qr = (const uint16_t*)a.q + tok * a.ld_q + (int64_t)hq * HD + 8 * g;
+#pragma unroll
+    for (int j = 0; j < HD / 16; ++j) qf[j] = *(const u32x4_t*)(qr + 16 * j);
+    RowInfo ri;
+    Pages pg{a.prefix_table, 0, a.prefix_len};
+    int first = s0;
+    if constexpr (MOD) {
+      ri.rel = a.positions ? (int)a.positions[tok] : 0;
+      ri.slope2 = a.slopes ? a.slopes[hq] * kLog2e : 0.f;
+      if (a.window > 0) {  // steps that lie behind every row's window are left out
+        const int64_t lo0 = (int64_t)ri.rel - a.window + 1;
+        int lo = (int)min(max(lo0, (int64_t)0), a.prefix_len);
+        if (!live) lo = (int)a.prefix_len;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) lo = min(lo, __shfl_xor(lo, d, 64));
+        __syncthreads();
+        if (lane == 0) s_lo[wave] = lo;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < C::W; ++i) lo = min(lo, s_lo[i]);
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        pg.lo = min((int64_t)lo, a.prefix_len - 1);
+        first = lo >= a.prefix_len ? s1 : max(s0, lo / C::SK);
+      }
+    }
+    f32x16_t o[HD / 32];
+    float m, l;
+    attend<DT, C, MOD, true>(a, smem, pg, kvh, first, max(first, s1), a.prefix_len, 0, live, a.prefix_len - 1, ri, qf,
+                             nullptr, bad, o, m, l);
+    if (kg == 0 && live)
+      store_part<HD>(parts, a.nkv, (int)(w - prefix_first_wg(pp, x)), kvh, row0 + ln, g, o, m, l);
+  }
+  if (bad && lane == 0) atomicOr(a.status, PE_ERR_INDEX);
+}
+
+// ---------------------------------------------------------------------------
+// The sequences' own keys
+// ---------------------------------------------------------------------------
+// Workgroup = (sequence, KV head, key split of kps keys, block of NT row tiles).
+// A sequence of one split joins the prefix's parts of its rows to its own and
+// writes the output; otherwise each split is a part and paged_join_kernel does.
+template <int DT, int HD>
+__device__ __forceinline__ void write_out(const PagedAttn& a, int64_t tok, int hq, int g, const f32x16_t (&o)[HD / 32],
+                                          float l) {
+  typedef typename Elem<DT>::T Te;
+  Te* dst = (Te*)a.out + tok * a.ld_out + (int64_t)hq * HD + 4 * g;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int h = 0; h < HD / 32; ++h)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float v[4] = {o[h][4 * c] * inv, o[h][4 * c + 1] * inv, o[h][4 * c + 2] * inv, o[h][4 * c + 3] * inv};
+      Vec4<DT>::store(dst + 32 * h + 8 * c, v);
+    }
+}
+
+template <int DT, typename C, bool MOD>
+__global__ __launch_bounds__(64 * C::W, 2) void paged_seq_kernel(PagedAttn a, PagedPrefix pp, PagedParts parts,
+                                                                 int64_t kps, int nsplit, int nblk) {
+  constexpr int HD = C::HD;
+  __shared__ __align__(1024) uint8_t smem[C::kSmem];
+  __shared__ int s_npos[MOD ? 64 * PE_TREE_MAX_WORDS : 1];
+  __shared__ int s_lo[C::W];
+  int64_t item = xcd_item(blockIdx.x, gridDim.x);
+  const int blk = (int)(item % nblk);
+  item /= nblk;
+  const int split = (int)(item % nsplit);
+  item /= nsplit;
+  const int kvh = (int)(item % a.nkv), b = (int)(item / a.nkv);
+  const PagedSeq s = paged_seq(a, b);
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  if (!s.ok) {
+    if (s.err && tid == 0 && kvh == 0 && split == 0 && blk == 0) atomicOr(a.status, s.err);
+    return;
+  }
+  const int G = a.nh / a.nkv, T = s.rows;
+  const int64_t R = (int64_t)T * G, P = s.priv, S = P + T;
+  const int64_t blk0 = (int64_t)blk * (32 * C::NT);
+  const int my_splits = (int)((S + kps - 1) / kps);
+  if (blk0 >= R || split >= my_splits) return;
+  const int ln = lane & 31, g = lane >> 5, tile = wave % C::NT, kg = wave / C::NT;
+  const bool tree = a.mask_mode == PE_MASK_TREE;
+  const int64_t row0 = blk0 + 32 * tile;
+  const bool live = row0 < R;
+  const int64_t row = min(row0 + ln, R - 1);
+  const int t = (int)(row / G);
+  const int hq = kvh * G + (int)(row - (int64_t)t * G);
+  const int64_t tok = s.row0 + t;
+  u32x4_t qf[HD / 16];
+  const uint16_t* qr = (const uint16_t*)a.q + tok * a.ld_q + (int64_t)hq * HD + 8 * g;
+#pragma unroll
+  for (int j = 0; j < HD / 16; ++j) qf[j] = *(const u32x4_t*)(qr + 16 * j);
+  RowInfo ri;
+  ri.node = t;
+#pragma unroll
+  for (int w = 0; w < PE_TREE_MAX_WORDS; ++w) ri.nb[w] = tree && w < a.words ? a.bits[tok * a.words + w] : 0ull;
+  // the keys some row of the block sees end at hi; of this wave's tile, at last_key
+  const int t_blk = (int)min((int64_t)T - 1, (blk0 + 32 * C::NT - 1) / G);
+  const int t_tile = (int)min((int64_t)T - 1, (row0 + 31) / G);
+  Pages pg{a.block_table + b * a.ld_table, 0, tree ? S : P + t_blk + 1};
+  const int64_t last_key = tree ? S - 1 : P + t_tile;
+  if constexpr (MOD) {
+    ri.rel = a.positions ? (int)(a.positions[tok] - a.prefix_len) : 0;
+    ri.slope2 = a.slopes ? a.slopes[hq] * kLog2e : 0.f;
+    if (a.positions && tree)
+      for (int u = tid; u < T; u += 64 * C::W) s_npos[u] = (int)(a.positions[s.row0 + u] - a.prefix_len);
+    if (a.window > 0) {
+      int lo = (int)min(max((int64_t)ri.rel - a.window + 1, (int64_t)0), P);
+      if (!live) lo = (int)P;
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) lo = min(lo, __shfl_xor(lo, d, 64));
+      if (lane == 0) s_lo[wave] = lo;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < C::W; ++i) lo = min(lo, s_lo[i]);
+      pg.lo = __builtin_amdgcn_readfirstlane(lo);
+    }
+  }
+  const int64_t k0 = (int64_t)split * kps, k1 = min(pg.hi, k0 + kps);
+  const int s1 = (int)((k1 + C::SK - 1) / C::SK);
+  const int s0 = (int)max(k0 / C::SK, pg.lo / C::SK);
+  bool bad = false;
+  f32x16_t o[HD / 32];
+  float m, l;
+  attend<DT, C, MOD, false>(a, smem, pg, kvh, s0, max(s0, s1), P, T, live, last_key, ri, qf, s_npos, bad, o, m, l);
+  if (bad && lane == 0) atomicOr(a.status, PE_ERR_INDEX);
+  if (kg != 0 || row0 + ln >= R) return;
+  const int64_t grow = (int64_t)s.row0 * G + row;  // the row among the whole batch's
+  if (my_splits > 1) {
+    store_part<HD>(parts, a.nkv, parts.pre_parts + split, kvh, grow, g, o, m, l);
+    return;
+  }
+  if (parts.pre_parts > 0) {
+    const int n = prefix_parts_of(pp, (int64_t)kvh * pp.nblk + grow / pp.block_rows);
+    for (int p = 0; p < n; ++p) {
+      const float2 ml = ((const float2*)parts.ml)[((int64_t)p * a.nkv + kvh) * parts.tiles * 32 + grow];
+      const float mx = fmaxf(m, ml.x);
+      const float a0 = __builtin_amdgcn_exp2f(m - mx), a1 = __builtin_amdgcn_exp2f(ml.x - mx);
+      m = mx;
+      l = a0 * l + a1 * ml.y;
+      const float* src = parts.o + part_tile<HD>(parts, a.nkv, p, kvh, grow >> 5) + ((grow & 31) + 32 * g) * 4;
+#pragma unroll
+      for (int h = 0; h < HD / 32; ++h)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const f32x4_t o1 = *(const f32x4_t*)(src + (4 * h + c) * 256);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[h][4 * c + i] = a0 * o[h][4 * c + i] + a1 * o1[i];
+        }
+    }
+  }
+  write_out<DT, HD>(a, tok, hq, g, o, l);
+}
+
+// Joins the parts of the sequences whose own keys are split: one thread per
+// (row, four dims), the prefix's parts first, then the splits in key order.
+template <int DT, int HD>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefix pp, PagedParts parts, int64_t kps) {
+  const int b = blockIdx.z, kvh = blockIdx.y;
+  const PagedSeq s = paged_seq(a, b);
+  if (!s.ok) return;
+  const int my_splits = (int)((s.priv + s.rows + kps - 1) / kps);
+  const int G = a.nh / a.nkv;
+  const int64_t R = (int64_t)s.rows * G;
+  // thread order inside a block: rows fastest, as a part's tile is stored
+  const int64_t row = (int64_t)blockIdx.x * (1024 / HD) + threadIdx.x % (1024 / HD);
+  const int piece = threadIdx.x / (1024 / HD);  // dims 4 piece .. + 3
+  if (my_splits <= 1 || row >= R) return;
+  const int64_t grow = (int64_t)s.row0 * G + row;
+  const int npre = parts.pre_parts > 0 ? prefix_parts_of(pp, (int64_t)kvh * pp.nblk + grow / pp.block_rows) : 0;
+  const int at = (piece >> 1) * 256 + ((int)(grow & 31) + 32 * (piece & 1)) * 4;
+  float m = kPagedInitMax, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < npre + my_splits; ++i) {
+    const int p = i < npre ? i : parts.pre_parts + i - npre;
+    const float2 ml = ((const float2*)parts.ml)[((int64_t)p * a.nkv + kvh) * parts.tiles * 32 + grow];
+    const f32x4_t v = *(const f32x4_t*)(parts.o + part_tile<HD>(parts, a.nkv, p, kvh, grow >> 5) + at);
+    const float mx = fmaxf(m, ml.x);
+    const float a0 = __builtin_amdgcn_exp2f(m - mx), a1 = __builtin_amdgcn_exp2f(ml.x - mx);
+    m = mx;
+    l = a0 * l + a1 * ml.y;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[d] = a0 * o[d] + a1 * v[d];
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+  typedef typename Elem<DT>::T Te;
+  const int64_t tok = grow / G;
+  const int hq = kvh * G + (int)(grow - tok * G);
+  Vec4<DT>::store((Te*)a.out + tok * a.ld_out + (int64_t)hq * HD + 4 * piece, v);
+}
+
+// ------------------------------------------------------------------ plans
+constexpr int kCus = 256;
+
+// Row tiles of a workgroup and the keys of a step, by the row tiles there are
+// (see the kernels' configurations).
+struct Shape {
+  int kind, tiles, step;
+};
+Shape shape_of(int64_t tiles) {
+  if (tiles > 4) return {0, 8, 64};
+  if (tiles > 2) return {1, 4, 64};
+  if (tiles > 1) return {2, 2, 64};
+  return {3, 1, 64};
+}
+
+struct Plan {
+  PagedPrefix pp;
+  Shape pre, seq;
+  int64_t pre_wgs, kps, o_bytes, ml_bytes;
+  int nsplit, seq_blocks, parts;
+  PagedParts pt;
+};
+
+Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int64_t max_len, int64_t prefix_len) {
+  Plan p;
+  const int G = nh / nkv;
+  p.pt.tiles = (M * G + 31) / 32 + 1;  // a tile row past the last: splits of the last rows
+  p.pp = PagedPrefix{0, 1, 1, 1, 32};
+  p.pre = Shape{0, 8, 64};
+  p.pre_wgs = 0;
+  p.pt.pre_parts = 0;
+  if (prefix_len > 0) {
+    const int64_t tiles = (M * G + 31) / 32;
+    p.pre = shape_of(tiles);
+    p.pp.nblk = (int)((tiles + p.pre.tiles - 1) / p.pre.tiles);
+    p.pp.block_rows = 32 * p.pre.tiles;
+    p.pp.steps = (prefix_len + p.pre.step - 1) / p.pre.step;
+    p.pp.total = nkv * p.pp.nblk * p.pp.steps;
+    const int64_t room = kCus * (p.pre.kind == 0 ? 1 : 2);
+    const int64_t want = std::max<int64_t>(8, std::min<int64_t>(room, p.pp.total / 4));
+    p.pp.per = (p.pp.total + want - 1) / want;
+    p.pre_wgs = (p.pp.total + p.pp.per - 1) / p.pp.per;
+    p.pt.pre_parts = (int)((p.pp.steps - 1) / p.pp.per) + 2;
+  }
+  const int64_t rt = ((int64_t)max_rows * G + 31) / 32;
+  p.seq = shape_of(rt);
+  p.seq_blocks = (int)((rt + p.seq.tiles - 1) / p.seq.tiles);
+  const int64_t keys = max_len - prefix_len + max_rows;
+  const int64_t wgs = (int64_t)batch * nkv * p.seq_blocks;
+  int64_t ns = std::max<int64_t>(1, std::min<int64_t>(2 * kCus / wgs, keys / 256));
+  p.kps = (((keys + ns - 1) / ns + 63) / 64) * 64;
+  p.nsplit = (int)((keys + p.kps - 1) / p.kps);
+  p.parts = p.pt.pre_parts + (p.nsplit > 1 ? p.nsplit : 0);
+  p.o_bytes = (int64_t)p.parts * nkv * p.pt.tiles * 32 * hd * 4;
+  p.ml_bytes = (int64_t)p.parts * nkv * p.pt.tiles * 32 * 8;
+  return p;
+}
+
+template <int DT, int HD, bool MOD>
+void launch_prefix(const Plan& p, const PagedAttn& a, hipStream_t st) {
+  const unsigned n = (unsigned)p.pre_wgs;
+  switch (p.pre.kind) {
+    case 0: paged_prefix_kernel<DT, Cfg<HD, 8, 1, 2, 4>, MOD><<<n, 512, 0, st>>>(a, p.pp, p.pt); break;
+    case 1: paged_prefix_kernel<DT, Cfg<HD, 4, 1, 2, 2>, MOD><<<n, 256, 0, st>>>(a, p.pp, p.pt); break;
+    case 2: paged_prefix_kernel<DT, Cfg<HD, 4, 2, 1, 2>, MOD><<<n, 256, 0, st>>>(a, p.pp, p.pt); break;
+    default: paged_prefix_kernel<DT, Cfg<HD, 2, 2, 1, 2>, MOD><<<n, 128, 0, st>>>(a, p.pp, p.pt); break;
+  }
+}
+template <int DT, int HD, bool MOD>
+void launch_seq(const Plan& p, const PagedAttn& a, hipStream_t st) {
+  const unsigned n = (unsigned)((int64_t)a.batch * a.nkv * p.nsplit * p.seq_blocks);
+  switch (p.seq.kind) {
+    case 0: paged_seq_kernel<DT, Cfg<HD, 8, 1, 2, 4>, MOD><<<n, 512, 0, st>>>(a, p.pp, p.pt, p.kps, p.nsplit, p.seq_blocks); break;
+    case 1: paged_seq_kernel<DT, Cfg<HD, 4, 1, 2, 2>, MOD><<<n, 256, 0, st>>>(a, p.pp, p.pt, p.kps, p.nsplit, p.seq_blocks); break;
+    case 2: paged_seq_kernel<DT, Cfg<HD, 4, 2, 1, 2>, MOD><<<n, 256, 0, st>>>(a, p.pp, p.pt, p.kps, p.nsplit, p.seq_blocks); break;
+    default: paged_seq_kernel<DT, Cfg<HD, 2, 2, 1, 2>, MOD><<<n, 128, 0, st>>>(a, p.pp, p.pt, p.kps, p.nsplit, p.seq_blocks); break;
+  }
+}
+
+template <int DT, int HD, bool MOD>
+int launch_all(const Plan& p, const PagedAttn& a, hipStream_t st) {
+  if (a.prefix_len > 0) {
+    launch_prefix<DT, HD, MOD>(p, a, st);
+    PE_CHECK_LAUNCH();
+  }
+  launch_seq<DT, HD, MOD>(p, a, st);
+  PE_CHECK_LAUNCH();
+  if (p.nsplit > 1) {
+    const int64_t rows = (int64_t)a.max_rows * (a.nh / a.nkv);
+    paged_join_kernel<DT, HD><<<dim3(pe_cdiv(rows, 1024 / HD), a.nkv, a.batch), 256, 0, st>>>(a, p.pp, p.pt, p.kps);
+    PE_CHECK_LAUNCH();
+  }
+  return PE_OK;
+}
+
+}  // namespace
+
+int64_t pe_internal_paged_mfma_bytes(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int64_t max_len,
+                                     int64_t prefix_len) {
+  const Plan p = make_plan(M, batch, nh, nkv, hd, max_rows, max_len, prefix_len);
+  return p.o_bytes + p.ml_bytes;
+}
+
+int pe_internal_paged_mfma(const PagedAttn& a, int dtype, void* workspace, int64_t workspace_bytes, hipStream_t st) {
+  Plan p = make_plan(a.M, a.batch, a.nh, a.nkv, a.hd, a.max_rows, a.max_len, a.prefix_len);
+  if (workspace_bytes < p.o_bytes + p.ml_bytes || (p.parts > 0 && !workspace)) return PE_ERR_WORKSPACE;
+  if ((uintptr_t)workspace & 15) return PE_ERR_ARG;
+  p.pt.o = (float*)workspace;
+  p.pt.ml = (float*)((char*)workspace + p.o_bytes);
+  const bool mod = a.softcap > 0.f || a.slopes || a.window > 0;
+#define PE_GO(DT, HD) return mod ? launch_all<DT, HD, true>(p, a, st) : launch_all<DT, HD, false>(p, a, st)
+  if (dtype == PE_DTYPE_BF16) {
+    if (a.hd == 128) PE_GO(PE_DTYPE_BF16, 128);
+    PE_GO(PE_DTYPE_BF16, 64);
+  }
+  if (a.hd == 128) PE_GO(PE_DTYPE_F16, 128);
+  PE_GO(PE_DTYPE_F16, 64);
+#undef PE_GO
+}
