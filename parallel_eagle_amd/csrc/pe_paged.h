@@ -74,12 +74,11 @@ struct PagedParts {
 // sequence, so all workgroups do the same amount and a block is covered by a
 // few of them, its parts.
 struct PagedPrefix {
-  int64_t total, per, steps;
-  int nblk, block_rows;
+  uint32_t total, per, steps, nblk, block_rows;
 };
 
-__device__ __forceinline__ int64_t prefix_first_wg(const PagedPrefix& p, int64_t block) { return block * p.steps / p.per; }
-__device__ __forceinline__ int prefix_parts_of(const PagedPrefix& p, int64_t block) {
+__device__ __forceinline__ uint32_t prefix_first_wg(const PagedPrefix& p, uint32_t block) { return block * p.steps / p.per; }
+__device__ __forceinline__ int prefix_parts_of(const PagedPrefix& p, uint32_t block) {
   return (int)((block * p.steps + p.steps - 1) / p.per - prefix_first_wg(p, block)) + 1;
 }
 

@@ -76,41 +76,40 @@ struct RowInfo {
   int64_t node;   // causal: its token's index among the sequence's new rows; tree: unused
   int rel;        // its position - the position of key 0 of the list (MOD)
   float slope2;   // slope * log2 e (MOD)
-  uint64_t nb[PE_TREE_MAX_WORDS];
+  int lo, tile_lo;  // first cached key its window holds; the largest of the tile's (MOD)
+  uint64_t nb0, nb1, nb2, nb3;  // ancestor bits (named: an indexed array would live in scratch memory)
 };
+static_assert(PE_TREE_MAX_WORDS == 4, "one field per word");
 
-// The configuration of a workgroup: W waves = NT row tiles x NK key groups, each
-// wave SB 32-key blocks of a step, a ring of ST steps in LDS filled straight
-// from global memory (ST - 1 of them in flight while one is multiplied).
-template <int HD_, int W_, int NK_, int SB_, int ST_>
+// The configuration of a workgroup: W waves of one 32-row tile each, SB 32-key
+// blocks in a step, a ring of ST steps in LDS filled straight from global memory
+// (ST - 1 of them in flight while one is multiplied).
+template <int HD_, int W_, int SB_, int ST_>
 struct Cfg {
-  static constexpr int HD = HD_, W = W_, NK = NK_, SB = SB_, ST = ST_;
-  static constexpr int NT = W / NK;
-  static constexpr int SK = 32 * NK * SB;            // keys of a step
-  static constexpr int kHalf = SK * HD * 2;          // bytes of a step's K (and of its V)
+  static constexpr int HD = HD_, W = W_, SB = SB_, ST = ST_;
+  static constexpr int SK = 32 * SB;                    // keys of a step
+  static constexpr int kHalf = SK * HD * 2;             // bytes of a step's K (and of its V)
   static constexpr int kStep = 2 * kHalf;
-  static constexpr int kChunks = 2 * SK / 16 / W;    // 16-key pieces of K or V a wave loads per step
+  static constexpr int kChunks = 2 * SK / 16 / W;       // 16-key pieces of K or V a wave loads per step
   static constexpr int kPerChunk = 16 * HD * 2 / 1024;  // load instructions of one
   static constexpr int kLoads = kChunks * kPerChunk;
-  static constexpr int kMergeRow = HD / 2 + 4;       // floats per lane of a key group's hand-over (16-byte rows)
-  static constexpr int kMerge = NT * 64 * kMergeRow * 4;
-  static constexpr int kSmem = ST * kStep > kMerge || NK == 1 ? ST * kStep : kMerge;
+  static constexpr int kSmem = ST * kStep;
   static_assert(2 * SK / 16 % W == 0, "whole pieces per wave");
 };
 
 // One 64-bit-masked step's visibility, bit j: key kb0 + j. Tree rows see keys
 // below P and the nodes of their bits; causal rows those up to P + node.
-__device__ __forceinline__ uint64_t node_window(int64_t kb0, int64_t P, const uint64_t* nb) {
+__device__ __forceinline__ uint64_t node_window(int64_t kb0, int64_t P, const RowInfo& r) {
   const int64_t off = kb0 - P;  // node index of key kb0
   if (off <= -64) return ~0ull;
   if (off < 0) {
     const int j0 = (int)(-off);
-    return ((1ull << j0) - 1) | (nb[0] << j0);
+    return ((1ull << j0) - 1) | (r.nb0 << j0);
   }
   if (off >= 64 * PE_TREE_MAX_WORDS) return 0ull;
   const int wi = (int)(off >> 6), sh = (int)(off & 63);
-  const uint64_t a = wi == 0 ? nb[0] : wi == 1 ? nb[1] : wi == 2 ? nb[2] : nb[3];
-  const uint64_t b = wi == 0 ? nb[1] : wi == 1 ? nb[2] : wi == 2 ? nb[3] : 0ull;
+  const uint64_t a = wi == 0 ? r.nb0 : wi == 1 ? r.nb1 : wi == 2 ? r.nb2 : r.nb3;
+  const uint64_t b = wi == 0 ? r.nb1 : wi == 1 ? r.nb2 : wi == 2 ? r.nb3 : 0ull;
   return sh ? (a >> sh) | (b << (64 - sh)) : a;
 }
 __device__ __forceinline__ uint64_t below(int64_t n) {  // bits 0 .. n - 1
@@ -118,11 +117,10 @@ __device__ __forceinline__ uint64_t below(int64_t n) {  // bits 0 .. n - 1
 }
 
 // The keys [s0 SK, s1 SK) of a list for the workgroup's row tiles: O^T, m, l of
-// the wave's tile over its key group, then joined over the key groups (valid in
-// key group 0). `P`: the list's cached keys, new rows follow (PRE: no new rows).
-// Every step's keys outside [pg.lo, pg.hi) are masked; `whole_to` is the first
-// key that some row of the tile may not see (tree or causal rows). npos (LDS):
-// positions of the new rows relative to key 0 (tree rows with MOD).
+// the wave's tile. `P`: the list's cached keys, new rows follow (PRE: no new rows).
+// Keys outside [pg.lo, pg.hi) are masked, steps past last_key (the last that a
+// row of the tile sees) skipped. npos (LDS): positions of the new rows relative
+// to key 0 (MOD, where distances count).
 template <int DT, typename C, bool MOD, bool PRE>
 __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const Pages& pg, int kvh, int s0, int s1,
                                        int64_t P, int new_rows, bool live, int64_t last_key, const RowInfo& ri,
@@ -131,7 +129,6 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
   constexpr int HD = C::HD, SB = C::SB;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int ln = lane & 31, g = lane >> 5;
-  const int kg = wave / C::NT;
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
   typedef const __attribute__((address_space(4))) int32_t* const_i32;  // read through the scalar cache
   const const_i32 tab = (const_i32)(uintptr_t)uniform_ptr((const uint16_t*)pg.table);
@@ -185,15 +182,15 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
   const bool tree = a.mask_mode == PE_MASK_TREE;
   const float cap_in = MOD && a.softcap > 0.f ? 2.f * scale2 / a.softcap : 0.f, cap_out = a.softcap * kLog2e;
 
-  __syncthreads();  // the buffers' and hand-over's last readers are done
-  __builtin_amdgcn_s_waitcnt(0);  // Q has landed: no later wait of the compiler's covers the ring's loads
   if (s0 < s1) ask(s0);
+  __syncthreads();  // the buffers' and hand-over's last readers are done
 #pragma unroll
   for (int i = 0; i < C::ST - 1; ++i)
     if (s0 + i < s1) {
       issue(s0 + i);
       if (s0 + i + 1 < s1) ask(s0 + i + 1);
     }
+  __builtin_amdgcn_s_waitcnt(0);  // Q has landed: no later wait of the compiler's covers the ring's loads
   for (int s = s0; s < s1; ++s) {
     if (s1 - 1 - s >= C::ST - 2) wait_vm<(C::ST - 2) * C::kLoads>();
     else wait_vm<0>();
@@ -204,9 +201,9 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
       issue(s + C::ST - 1);
       if (s + C::ST < s1) ask(s + C::ST);
     }
-    const int64_t kb0 = (int64_t)s * C::SK + kg * 32 * SB;
+    const int64_t kb0 = (int64_t)s * C::SK;
     if (!live || kb0 > last_key) continue;  // wave-uniform: the tile sees no key of this step
-    const uint8_t* kbp = smem + (s % C::ST) * C::kStep + kg * 32 * SB * HD * 2;
+    const uint8_t* kbp = smem + (s % C::ST) * C::kStep;
     const uint8_t* vbp = kbp + C::kHalf;
     f32x16_t sc[SB];
 #pragma unroll
@@ -237,31 +234,35 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
 #pragma unroll
           for (int i = 0; i < 16; ++i) sc[sb][i] *= scale2;
       }
-      const bool listed = node_step && tree;  // distances of new rows come from their positions
-      if (a.slopes || a.window > 0) {
-        const int d0 = ri.rel - (int)kb0 - 4 * g;
-        const int64_t w = a.window;
+      const int d0 = ri.rel - (int)kb0 - 4 * g;  // distance of key kb0 + 4 g
+      if (node_step && tree && npos) {  // new rows lie where their positions say
 #pragma unroll
         for (int sb = 0; sb < SB; ++sb)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int off = 32 * sb + 8 * (i >> 2) + (i & 3);
-            int dist = d0 - off;
-            if (listed) {
-              const int64_t u = kb0 + off + 4 * g - P;
-              const int np = npos[u < 0 ? 0 : u < new_rows ? (int)u : new_rows - 1];
-              dist = u < 0 ? dist : ri.rel - np;
-            }
+            const int u = (int)(kb0 - P) + off + 4 * g;
+            const int np = npos[max(0, min(u, new_rows - 1))];
+            const int dist = u < 0 ? d0 - off : ri.rel - np;
             sc[sb][i] = fmaf(-ri.slope2, (float)dist, sc[sb][i]);
-            if (w > 0) sc[sb][i] = (int64_t)dist < w ? sc[sb][i] : -INFINITY;
+            if (a.window > 0) sc[sb][i] = dist < a.window ? sc[sb][i] : -INFINITY;
           }
+      } else if (a.slopes) {
+#pragma unroll
+        for (int sb = 0; sb < SB; ++sb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            sc[sb][i] = fmaf(-ri.slope2, (float)(d0 - (32 * sb + 8 * (i >> 2) + (i & 3))), sc[sb][i]);
       }
     }
-    const bool edge = node_step || kb0 + 32 * SB > pg.hi || kb0 < pg.lo;
+    bool edge = node_step || kb0 + 32 * SB > pg.hi || kb0 < pg.lo;
+    if constexpr (MOD) edge = edge || kb0 < ri.tile_lo;
     if (edge) {
       uint64_t win = ~0ull;
-      if constexpr (!PRE) win = tree ? node_window(kb0, P, ri.nb) : below(P + ri.node + 1 - kb0);
-      win &= below(pg.hi - kb0) & ~below(pg.lo - kb0);
+      if constexpr (!PRE) win = tree ? node_window(kb0, P, ri) : below(P + ri.node + 1 - kb0);
+      int64_t lo = pg.lo;
+      if constexpr (MOD) lo = max(lo, (int64_t)ri.lo);
+      win &= below(pg.hi - kb0) & ~below(lo - kb0);
       win >>= 4 * g;
 #pragma unroll
       for (int sb = 0; sb < SB; ++sb)
@@ -320,52 +321,21 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
       }
     }
   }
-  if constexpr (C::NK > 1) {
-    // the key groups hand their (O, m, l) to group 0 in turn
-    const int tile = wave % C::NT;
-    float* mo = (float*)smem + (tile * 64 + lane) * C::kMergeRow;
-    for (int k = 1; k < C::NK; ++k) {
-      __syncthreads();
-      if (kg == k) {
-#pragma unroll
-        for (int h = 0; h < HD / 32; ++h)
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            *(f32x4_t*)&mo[16 * h + 4 * c] = f32x4_t{o[h][4 * c], o[h][4 * c + 1], o[h][4 * c + 2], o[h][4 * c + 3]};
-        mo[HD / 2] = m;
-        mo[HD / 2 + 1] = l;
-      }
-      __syncthreads();
-      if (kg == 0) {
-        const float m1 = mo[HD / 2], l1 = mo[HD / 2 + 1];
-        const float mx = fmaxf(m, m1);
-        const float a0 = __builtin_amdgcn_exp2f(m - mx), a1 = __builtin_amdgcn_exp2f(m1 - mx);
-        l = a0 * l + a1 * l1;
-        m = mx;
-#pragma unroll
-        for (int h = 0; h < HD / 32; ++h)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const f32x4_t o1 = *(const f32x4_t*)&mo[16 * h + 4 * c];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[h][4 * c + i] = a0 * o[h][4 * c + i] + a1 * o1[i];
-          }
-      }
-    }
-  }
 }
 
 // Work item of workgroup `b` of `n`: neighbours in the sequence of items (which
 // share a KV head's keys) on one XCD (workgroup b starts on XCD b % 8).
-__device__ __forceinline__ int64_t xcd_item(int64_t b, int64_t n) { return n & 7 ? b : (b & 7) * (n >> 3) + (b >> 3); }
+__device__ __forceinline__ uint32_t xcd_item(uint32_t b, uint32_t n) {
+  return n & 7 ? b : (b & 7) * (n >> 3) + (b >> 3);
+}
 
 template <int HD>
-__device__ __forceinline__ int64_t part_tile(const PagedParts& p, int nkv, int part, int kvh, int64_t tile) {
+__device__ __forceinline__ int64_t part_tile(const PagedParts& p, int nkv, int part, int kvh, uint32_t tile) {
   return (((int64_t)part * nkv + kvh) * p.tiles + tile) * (32 * HD);
 }
 
 template <int HD>
-__device__ __forceinline__ void store_part(const PagedParts& p, int nkv, int part, int kvh, int64_t row, int g,
+__device__ __forceinline__ void store_part(const PagedParts& p, int nkv, int part, int kvh, uint32_t row, int g,
                                            const f32x16_t (&o)[HD / 32], float m, float l) {
   float* dst = p.o + part_tile<HD>(p, nkv, part, kvh, row >> 5) + ((row & 31) + 32 * g) * 4;
 #pragma unroll
@@ -379,6 +349,30 @@ __device__ __forceinline__ void store_part(const PagedParts& p, int nkv, int par
   }
 }
 
+// The lane's row's first cached key inside its window (ri.lo), the last of the
+// tile's (ri.tile_lo) and the first of the workgroup's (returned); `cached` keys.
+template <int W>
+__device__ __forceinline__ int window_lo(const PagedAttn& a, RowInfo& ri, int cached, bool live, int* s_lo) {
+  ri.lo = ri.tile_lo = 0;
+  if (a.window == 0) return 0;
+  ri.lo = (int)min(max((int64_t)ri.rel - a.window + 1, (int64_t)0), (int64_t)cached);
+  int lo = live ? ri.lo : cached, hi = ri.lo;
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    lo = min(lo, __shfl_xor(lo, d, 64));
+    hi = max(hi, __shfl_xor(hi, d, 64));
+  }
+  ri.tile_lo = __builtin_amdgcn_readfirstlane(hi);
+  if constexpr (W > 1) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s_lo[threadIdx.x >> 6] = lo;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < W; ++i) lo = min(lo, s_lo[i]);
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
 // ---------------------------------------------------------------------------
 // The prefix
 // ---------------------------------------------------------------------------
@@ -388,22 +382,21 @@ __global__ __launch_bounds__(64 * C::W, 2) void paged_prefix_kernel(PagedAttn a,
   __shared__ __align__(1024) uint8_t smem[C::kSmem];
   __shared__ int s_lo[C::W];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int ln = lane & 31, g = lane >> 5, tile = wave % C::NT, kg = wave / C::NT;
-  const int G = a.nh / a.nkv;
-  const int64_t R = a.M * G;
-  const int64_t w = xcd_item(blockIdx.x, gridDim.x);
-  const int64_t uend = min(pp.total, (w + 1) * pp.per);
+  const int ln = lane & 31, g = lane >> 5, tile = wave;
+  const uint32_t G = (uint32_t)(a.nh / a.nkv), R = (uint32_t)a.M * G;
+  const uint32_t w = xcd_item(blockIdx.x, gridDim.x);
+  const uint32_t uend = min(pp.total, (w + 1) * pp.per);
   bool bad = false;
-  for (int64_t u = w * pp.per; u < uend;) {
-    const int64_t x = u / pp.steps;
+  for (uint32_t u = w * pp.per; u < uend;) {
+    const uint32_t x = u / pp.steps;
     const int s0 = (int)(u - x * pp.steps);
     const int s1 = (int)min(pp.steps, s0 + (uend - u));
     u += s1 - s0;
     const int kvh = (int)(x / pp.nblk);
-    const int64_t row0 = (x - (int64_t)kvh * pp.nblk) * pp.block_rows + 32 * tile;
-    const bool live = row0 < R;
-    const int64_t row = min(row0 + ln, R - 1), tok = row / G;
-    const int hq = kvh * G + (int)(row - tok * G);
+    const uint32_t blk0 = (x - kvh * pp.nblk) * pp.block_rows, row0 = blk0 + 32 * tile;
+    const bool live = row0 < min(blk0 + pp.block_rows, R);
+    const uint32_t row = min(row0 + ln, R - 1), tok = row / G;
+    const int hq = (int)(kvh * G + (row - tok * G));
     u32x4_t qf[HD / 16];
     const uint16_t* qr = (const uint16_t*)a.q + tok * a.ld_q + (int64_t)hq * HD + 8 * g;
 #pragma unroll
@@ -414,27 +407,15 @@ __global__ __launch_bounds__(64 * C::W, 2) void paged_prefix_kernel(PagedAttn a,
     if constexpr (MOD) {
       ri.rel = a.positions ? (int)a.positions[tok] : 0;
       ri.slope2 = a.slopes ? a.slopes[hq] * kLog2e : 0.f;
-      if (a.window > 0) {  // steps that lie behind every row's window are left out
-        const int64_t lo0 = (int64_t)ri.rel - a.window + 1;
-        int lo = (int)min(max(lo0, (int64_t)0), a.prefix_len);
-        if (!live) lo = (int)a.prefix_len;
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) lo = min(lo, __shfl_xor(lo, d, 64));
-        __syncthreads();
-        if (lane == 0) s_lo[wave] = lo;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < C::W; ++i) lo = min(lo, s_lo[i]);
-        lo = __builtin_amdgcn_readfirstlane(lo);
-        pg.lo = min((int64_t)lo, a.prefix_len - 1);
-        first = lo >= a.prefix_len ? s1 : max(s0, lo / C::SK);
-      }
+      const int lo = window_lo<C::W>(a, ri, (int)a.prefix_len, live, s_lo);
+      pg.lo = min((int64_t)lo, a.prefix_len - 1);
+      if (lo > 0) first = lo >= a.prefix_len ? s1 : max(s0, lo / C::SK);  // steps behind every row's window
     }
     f32x16_t o[HD / 32];
     float m, l;
     attend<DT, C, MOD, true>(a, smem, pg, kvh, first, max(first, s1), a.prefix_len, 0, live, a.prefix_len - 1, ri, qf,
                              nullptr, bad, o, m, l);
-    if (kg == 0 && live)
+    if (live)
       store_part<HD>(parts, a.nkv, (int)(w - prefix_first_wg(pp, x)), kvh, row0 + ln, g, o, m, l);
   }
   if (bad && lane == 0) atomicOr(a.status, PE_ERR_INDEX);
@@ -463,35 +444,44 @@ __device__ __forceinline__ void write_out(const PagedAttn& a, int64_t tok, int h
 
 template <int DT, typename C, bool MOD>
 __global__ __launch_bounds__(64 * C::W, 2) void paged_seq_kernel(PagedAttn a, PagedPrefix pp, PagedParts parts,
-                                                                 int64_t kps, int nsplit, int nblk) {
+                                                                 uint32_t kps, int nsplit, int nblk,
+                                                                 uint32_t block_rows) {
   constexpr int HD = C::HD;
   __shared__ __align__(1024) uint8_t smem[C::kSmem];
   __shared__ int s_npos[MOD ? 64 * PE_TREE_MAX_WORDS : 1];
   __shared__ int s_lo[C::W];
-  int64_t item = xcd_item(blockIdx.x, gridDim.x);
-  const int blk = (int)(item % nblk);
-  item /= nblk;
-  const int split = (int)(item % nsplit);
-  item /= nsplit;
-  const int kvh = (int)(item % a.nkv), b = (int)(item / a.nkv);
+  // blocks of one (split, sequence, KV head) on one XCD, neighbours in time;
+  // otherwise KV heads over the XCDs (workgroup i starts on XCD i % 8), so that
+  // sequences of different lengths load them alike, and the last splits, which
+  // short sequences leave empty, at the end
+  const uint32_t n1 = gridDim.x / (uint32_t)nblk;
+  uint32_t item = blockIdx.x, blk = 0;
+  if (nblk > 1) {
+    const uint32_t per = n1 & 7 ? 1 : 8, q = item / (per * nblk), r = item - q * per * nblk;
+    blk = r / per;
+    item = q * per + (r - blk * per);
+  }
+  const uint32_t sb = item / (uint32_t)a.nkv;
+  const int kvh = (int)(item - sb * a.nkv), split = (int)(sb / (uint32_t)a.batch), b = (int)(sb - split * a.batch);
   const PagedSeq s = paged_seq(a, b);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   if (!s.ok) {
     if (s.err && tid == 0 && kvh == 0 && split == 0 && blk == 0) atomicOr(a.status, s.err);
     return;
   }
-  const int G = a.nh / a.nkv, T = s.rows;
-  const int64_t R = (int64_t)T * G, P = s.priv, S = P + T;
-  const int64_t blk0 = (int64_t)blk * (32 * C::NT);
-  const int my_splits = (int)((S + kps - 1) / kps);
+  const int T = s.rows;
+  const uint32_t G = (uint32_t)(a.nh / a.nkv), R = T * G;
+  const int64_t P = s.priv, S = P + T;
+  const uint32_t blk0 = blk * block_rows;
+  const int my_splits = (int)(((uint32_t)S + kps - 1) / kps);
   if (blk0 >= R || split >= my_splits) return;
-  const int ln = lane & 31, g = lane >> 5, tile = wave % C::NT, kg = wave / C::NT;
+  const int ln = lane & 31, g = lane >> 5, tile = wave;
   const bool tree = a.mask_mode == PE_MASK_TREE;
-  const int64_t row0 = blk0 + 32 * tile;
-  const bool live = row0 < R;
-  const int64_t row = min(row0 + ln, R - 1);
+  const uint32_t row0 = blk0 + 32 * tile, row_end = min(blk0 + block_rows, R);
+  const bool live = row0 < row_end;
+  const uint32_t row = min(row0 + ln, R - 1);
   const int t = (int)(row / G);
-  const int hq = kvh * G + (int)(row - (int64_t)t * G);
+  const int hq = kvh * (int)G + (int)(row - t * G);
   const int64_t tok = s.row0 + t;
   u32x4_t qf[HD / 16];
   const uint16_t* qr = (const uint16_t*)a.q + tok * a.ld_q + (int64_t)hq * HD + 8 * g;
@@ -499,11 +489,17 @@ __global__ __launch_bounds__(64 * C::W, 2) void paged_seq_kernel(PagedAttn a, Pa
   for (int j = 0; j < HD / 16; ++j) qf[j] = *(const u32x4_t*)(qr + 16 * j);
   RowInfo ri;
   ri.node = t;
-#pragma unroll
-  for (int w = 0; w < PE_TREE_MAX_WORDS; ++w) ri.nb[w] = tree && w < a.words ? a.bits[tok * a.words + w] : 0ull;
+  ri.nb0 = ri.nb1 = ri.nb2 = ri.nb3 = 0ull;
+  if (tree) {
+    const uint64_t* bt = a.bits + tok * a.words;
+    ri.nb0 = bt[0];
+    if (a.words > 1) ri.nb1 = bt[1];
+    if (a.words > 2) ri.nb2 = bt[2];
+    if (a.words > 3) ri.nb3 = bt[3];
+  }
   // the keys some row of the block sees end at hi; of this wave's tile, at last_key
-  const int t_blk = (int)min((int64_t)T - 1, (blk0 + 32 * C::NT - 1) / G);
-  const int t_tile = (int)min((int64_t)T - 1, (row0 + 31) / G);
+  const int t_blk = min(T - 1, (int)((blk0 + block_rows - 1) / G));
+  const int t_tile = min(T - 1, (int)((row0 + 31) / G));
   Pages pg{a.block_table + b * a.ld_table, 0, tree ? S : P + t_blk + 1};
   const int64_t last_key = tree ? S - 1 : P + t_tile;
   if constexpr (MOD) {
@@ -511,34 +507,25 @@ __global__ __launch_bounds__(64 * C::W, 2) void paged_seq_kernel(PagedAttn a, Pa
     ri.slope2 = a.slopes ? a.slopes[hq] * kLog2e : 0.f;
     if (a.positions && tree)
       for (int u = tid; u < T; u += 64 * C::W) s_npos[u] = (int)(a.positions[s.row0 + u] - a.prefix_len);
-    if (a.window > 0) {
-      int lo = (int)min(max((int64_t)ri.rel - a.window + 1, (int64_t)0), P);
-      if (!live) lo = (int)P;
-#pragma unroll
-      for (int d = 32; d > 0; d >>= 1) lo = min(lo, __shfl_xor(lo, d, 64));
-      if (lane == 0) s_lo[wave] = lo;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < C::W; ++i) lo = min(lo, s_lo[i]);
-      pg.lo = __builtin_amdgcn_readfirstlane(lo);
-    }
+    pg.lo = window_lo<C::W>(a, ri, (int)(tree ? P : pg.hi - 1), live, s_lo);
   }
-  const int64_t k0 = (int64_t)split * kps, k1 = min(pg.hi, k0 + kps);
+  const int64_t k0 = (int64_t)split * kps, k1 = min(pg.hi, k0 + (int64_t)kps);
   const int s1 = (int)((k1 + C::SK - 1) / C::SK);
   const int s0 = (int)max(k0 / C::SK, pg.lo / C::SK);
   bool bad = false;
   f32x16_t o[HD / 32];
   float m, l;
-  attend<DT, C, MOD, false>(a, smem, pg, kvh, s0, max(s0, s1), P, T, live, last_key, ri, qf, s_npos, bad, o, m, l);
+  attend<DT, C, MOD, false>(a, smem, pg, kvh, s0, max(s0, s1), P, T, live, last_key, ri, qf,
+                            MOD && a.positions ? s_npos : nullptr, bad, o, m, l);
   if (bad && lane == 0) atomicOr(a.status, PE_ERR_INDEX);
-  if (kg != 0 || row0 + ln >= R) return;
-  const int64_t grow = (int64_t)s.row0 * G + row;  // the row among the whole batch's
+  if (row0 + ln >= row_end) return;
+  const uint32_t grow = (uint32_t)s.row0 * G + row;  // the row among the whole batch's
   if (my_splits > 1) {
     store_part<HD>(parts, a.nkv, parts.pre_parts + split, kvh, grow, g, o, m, l);
     return;
   }
   if (parts.pre_parts > 0) {
-    const int n = prefix_parts_of(pp, (int64_t)kvh * pp.nblk + grow / pp.block_rows);
+    const int n = prefix_parts_of(pp, kvh * pp.nblk + grow / pp.block_rows);
     for (int p = 0; p < n; ++p) {
       const float2 ml = ((const float2*)parts.ml)[((int64_t)p * a.nkv + kvh) * parts.tiles * 32 + grow];
       const float mx = fmaxf(m, ml.x);
@@ -562,91 +549,104 @@ __global__ __launch_bounds__(64 * C::W, 2) void paged_seq_kernel(PagedAttn a, Pa
 // Joins the parts of the sequences whose own keys are split: one thread per
 // (row, four dims), the prefix's parts first, then the splits in key order.
 template <int DT, int HD>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefix pp, PagedParts parts, int64_t kps) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefix pp, PagedParts parts, uint32_t kps) {
   const int b = blockIdx.z, kvh = blockIdx.y;
   const PagedSeq s = paged_seq(a, b);
   if (!s.ok) return;
-  const int my_splits = (int)((s.priv + s.rows + kps - 1) / kps);
-  const int G = a.nh / a.nkv;
-  const int64_t R = (int64_t)s.rows * G;
+  const int my_splits = (int)(((uint32_t)(s.priv + s.rows) + kps - 1) / kps);
+  const uint32_t G = (uint32_t)(a.nh / a.nkv), R = s.rows * G;
   // thread order inside a block: rows fastest, as a part's tile is stored
-  const int64_t row = (int64_t)blockIdx.x * (1024 / HD) + threadIdx.x % (1024 / HD);
+  const uint32_t row = blockIdx.x * (1024 / HD) + threadIdx.x % (1024 / HD);
   const int piece = threadIdx.x / (1024 / HD);  // dims 4 piece .. + 3
   if (my_splits <= 1 || row >= R) return;
-  const int64_t grow = (int64_t)s.row0 * G + row;
-  const int npre = parts.pre_parts > 0 ? prefix_parts_of(pp, (int64_t)kvh * pp.nblk + grow / pp.block_rows) : 0;
+  const uint32_t grow = (uint32_t)s.row0 * G + row;
+  const int npre = parts.pre_parts > 0 ? prefix_parts_of(pp, kvh * pp.nblk + grow / pp.block_rows) : 0;
   const int at = (piece >> 1) * 256 + ((int)(grow & 31) + 32 * (piece & 1)) * 4;
   float m = kPagedInitMax, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < npre + my_splits; ++i) {
-    const int p = i < npre ? i : parts.pre_parts + i - npre;
-    const float2 ml = ((const float2*)parts.ml)[((int64_t)p * a.nkv + kvh) * parts.tiles * 32 + grow];
-    const f32x4_t v = *(const f32x4_t*)(parts.o + part_tile<HD>(parts, a.nkv, p, kvh, grow >> 5) + at);
-    const float mx = fmaxf(m, ml.x);
-    const float a0 = __builtin_amdgcn_exp2f(m - mx), a1 = __builtin_amdgcn_exp2f(ml.x - mx);
-    m = mx;
-    l = a0 * l + a1 * ml.y;
+  constexpr int kAhead = 4;  // parts asked for before the first is joined
+  const int n = npre + my_splits;
+  for (int i0 = 0; i0 < n; i0 += kAhead) {
+    float2 ml[kAhead];
+    f32x4_t v[kAhead];
 #pragma unroll
-    for (int d = 0; d < 4; ++d) o[d] = a0 * o[d] + a1 * v[d];
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = min(i0 + k, n - 1), p = i < npre ? i : parts.pre_parts + i - npre;
+      ml[k] = ((const float2*)parts.ml)[((int64_t)p * a.nkv + kvh) * parts.tiles * 32 + grow];
+      v[k] = *(const f32x4_t*)(parts.o + part_tile<HD>(parts, a.nkv, p, kvh, grow >> 5) + at);
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (i0 + k >= n) break;
+      const float mx = fmaxf(m, ml[k].x);
+      const float a0 = __builtin_amdgcn_exp2f(m - mx), a1 = __builtin_amdgcn_exp2f(ml[k].x - mx);
+      m = mx;
+      l = a0 * l + a1 * ml[k].y;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) o[d] = a0 * o[d] + a1 * v[k][d];
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
   typedef typename Elem<DT>::T Te;
-  const int64_t tok = grow / G;
-  const int hq = kvh * G + (int)(grow - tok * G);
+  const uint32_t tok = grow / G;
+  const int hq = (int)(kvh * G + (grow - tok * G));
   Vec4<DT>::store((Te*)a.out + tok * a.ld_out + (int64_t)hq * HD + 4 * piece, v);
 }
 
 // ------------------------------------------------------------------ plans
 constexpr int kCus = 256;
+constexpr int kSeqWgs = 2048, kMinSplit = 256, kSplitRows = 8, kPrefixSteps = 4;
 
-// Row tiles of a workgroup and the keys of a step, by the row tiles there are
-// (see the kernels' configurations).
+// A launch's workgroups: which configuration, row tiles per block and how many
+// blocks hold `tiles` row tiles in equal shares.
 struct Shape {
-  int kind, tiles, step;
+  int kind, tiles, blocks;
 };
 Shape shape_of(int64_t tiles) {
-  if (tiles > 4) return {0, 8, 64};
-  if (tiles > 2) return {1, 4, 64};
-  if (tiles > 1) return {2, 2, 64};
-  return {3, 1, 64};
+  const int most = tiles > 4 ? 8 : tiles > 2 ? 4 : (int)tiles;
+  const int64_t blocks = (tiles + most - 1) / most;
+  return {most == 8 ? 0 : most == 4 ? 1 : most == 2 ? 2 : 3, (int)((tiles + blocks - 1) / blocks), (int)blocks};
 }
+// Keys of a step: 64, but 32 for 128-dim heads with at most four tiles.
+int step_keys(const Shape& s, int hd) { return s.kind == 0 || hd == 64 ? 64 : 32; }
 
 struct Plan {
   PagedPrefix pp;
   Shape pre, seq;
-  int64_t pre_wgs, kps, o_bytes, ml_bytes;
-  int nsplit, seq_blocks, parts;
+  int64_t units, pre_wgs, o_bytes, ml_bytes;
+  uint32_t kps;
+  int nsplit, parts;
   PagedParts pt;
 };
 
 Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int64_t max_len, int64_t prefix_len) {
   Plan p;
   const int G = nh / nkv;
-  p.pt.tiles = (M * G + 31) / 32 + 1;  // a tile row past the last: splits of the last rows
+  const int64_t tiles = (M * G + 31) / 32;
+  p.pt.tiles = tiles;
   p.pp = PagedPrefix{0, 1, 1, 1, 32};
-  p.pre = Shape{0, 8, 64};
-  p.pre_wgs = 0;
+  p.pre = Shape{0, 8, 1};
+  p.pre_wgs = p.units = 0;
   p.pt.pre_parts = 0;
   if (prefix_len > 0) {
-    const int64_t tiles = (M * G + 31) / 32;
     p.pre = shape_of(tiles);
-    p.pp.nblk = (int)((tiles + p.pre.tiles - 1) / p.pre.tiles);
-    p.pp.block_rows = 32 * p.pre.tiles;
-    p.pp.steps = (prefix_len + p.pre.step - 1) / p.pre.step;
-    p.pp.total = nkv * p.pp.nblk * p.pp.steps;
+    const int64_t steps = (prefix_len - 1) / step_keys(p.pre, hd) + 1;
+    const int64_t total = (int64_t)nkv * p.pre.blocks * steps;
+    p.units = total;
     const int64_t room = kCus * (p.pre.kind == 0 ? 1 : 2);
-    const int64_t want = std::max<int64_t>(8, std::min<int64_t>(room, p.pp.total / 4));
-    p.pp.per = (p.pp.total + want - 1) / want;
-    p.pre_wgs = (p.pp.total + p.pp.per - 1) / p.pp.per;
-    p.pt.pre_parts = (int)((p.pp.steps - 1) / p.pp.per) + 2;
+    const int64_t blocks = (int64_t)nkv * p.pre.blocks;
+    const int64_t want = std::min<int64_t>(room, std::max(blocks, total / kPrefixSteps));
+    p.pp = PagedPrefix{(uint32_t)total, (uint32_t)((total + want - 1) / want), (uint32_t)steps, (uint32_t)p.pre.blocks,
+                       (uint32_t)(32 * p.pre.tiles)};
+    p.pre_wgs = (total + p.pp.per - 1) / p.pp.per;
+    p.pt.pre_parts = (int)((steps - 1) / p.pp.per) + 2;
   }
-  const int64_t rt = ((int64_t)max_rows * G + 31) / 32;
-  p.seq = shape_of(rt);
-  p.seq_blocks = (int)((rt + p.seq.tiles - 1) / p.seq.tiles);
+  p.seq = shape_of(((int64_t)max_rows * G + 31) / 32);
   const int64_t keys = max_len - prefix_len + max_rows;
-  const int64_t wgs = (int64_t)batch * nkv * p.seq_blocks;
-  int64_t ns = std::max<int64_t>(1, std::min<int64_t>(2 * kCus / wgs, keys / 256));
-  p.kps = (((keys + ns - 1) / ns + 63) / 64) * 64;
+  const int64_t wgs = (int64_t)batch * nkv * p.seq.blocks;
+  const int64_t least = std::max<int64_t>(kMinSplit, kSplitRows * max_rows * G);
+  const int64_t ns = std::max<int64_t>(1, std::min<int64_t>(kSeqWgs / wgs, keys / least));
+  p.kps = (uint32_t)((((keys + ns - 1) / ns + 63) / 64) * 64);
   p.nsplit = (int)((keys + p.kps - 1) / p.kps);
   p.parts = p.pt.pre_parts + (p.nsplit > 1 ? p.nsplit : 0);
   p.o_bytes = (int64_t)p.parts * nkv * p.pt.tiles * 32 * hd * 4;
@@ -654,25 +654,32 @@ Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int6
   return p;
 }
 
+template <int HD> using Wide = Cfg<HD, 8, 2, 4>;
+template <int HD, int W> using Slim = Cfg<HD, W, HD == 128 ? 1 : 2, 3>;
+#define PE_ARG(...) __VA_ARGS__
+
 template <int DT, int HD, bool MOD>
 void launch_prefix(const Plan& p, const PagedAttn& a, hipStream_t st) {
   const unsigned n = (unsigned)p.pre_wgs;
   switch (p.pre.kind) {
-    case 0: paged_prefix_kernel<DT, Cfg<HD, 8, 1, 2, 4>, MOD><<<n, 512, 0, st>>>(a, p.pp, p.pt); break;
-    case 1: paged_prefix_kernel<DT, Cfg<HD, 4, 1, 2, 2>, MOD><<<n, 256, 0, st>>>(a, p.pp, p.pt); break;
-    case 2: paged_prefix_kernel<DT, Cfg<HD, 4, 2, 1, 2>, MOD><<<n, 256, 0, st>>>(a, p.pp, p.pt); break;
-    default: paged_prefix_kernel<DT, Cfg<HD, 2, 2, 1, 2>, MOD><<<n, 128, 0, st>>>(a, p.pp, p.pt); break;
+    case 0: paged_prefix_kernel<DT, Wide<HD>, MOD><<<n, 512, 0, st>>>(a, p.pp, p.pt); break;
+    case 1: paged_prefix_kernel<DT, Slim<HD, 4>, MOD><<<n, 256, 0, st>>>(a, p.pp, p.pt); break;
+    case 2: paged_prefix_kernel<DT, Slim<HD, 2>, MOD><<<n, 128, 0, st>>>(a, p.pp, p.pt); break;
+    default: paged_prefix_kernel<DT, Slim<HD, 1>, MOD><<<n, 64, 0, st>>>(a, p.pp, p.pt); break;
   }
 }
 template <int DT, int HD, bool MOD>
 void launch_seq(const Plan& p, const PagedAttn& a, hipStream_t st) {
-  const unsigned n = (unsigned)((int64_t)a.batch * a.nkv * p.nsplit * p.seq_blocks);
+  const unsigned n = (unsigned)((int64_t)a.batch * a.nkv * p.nsplit * p.seq.blocks);
+#define PE_SEQ(C, W) \
+  paged_seq_kernel<DT, C, MOD><<<n, 64 * W, 0, st>>>(a, p.pp, p.pt, p.kps, p.nsplit, p.seq.blocks, 32u * p.seq.tiles)
   switch (p.seq.kind) {
-    case 0: paged_seq_kernel<DT, Cfg<HD, 8, 1, 2, 4>, MOD><<<n, 512, 0, st>>>(a, p.pp, p.pt, p.kps, p.nsplit, p.seq_blocks); break;
-    case 1: paged_seq_kernel<DT, Cfg<HD, 4, 1, 2, 2>, MOD><<<n, 256, 0, st>>>(a, p.pp, p.pt, p.kps, p.nsplit, p.seq_blocks); break;
-    case 2: paged_seq_kernel<DT, Cfg<HD, 4, 2, 1, 2>, MOD><<<n, 256, 0, st>>>(a, p.pp, p.pt, p.kps, p.nsplit, p.seq_blocks); break;
-    default: paged_seq_kernel<DT, Cfg<HD, 2, 2, 1, 2>, MOD><<<n, 128, 0, st>>>(a, p.pp, p.pt, p.kps, p.nsplit, p.seq_blocks); break;
+    case 0: PE_SEQ(Wide<HD>, 8); break;
+    case 1: PE_SEQ(PE_ARG(Slim<HD, 4>), 4); break;
+    case 2: PE_SEQ(PE_ARG(Slim<HD, 2>), 2); break;
+    default: PE_SEQ(PE_ARG(Slim<HD, 1>), 1); break;
   }
+#undef PE_SEQ
 }
 
 template <int DT, int HD, bool MOD>
@@ -703,6 +710,10 @@ int pe_internal_paged_mfma(const PagedAttn& a, int dtype, void* workspace, int64
   Plan p = make_plan(a.M, a.batch, a.nh, a.nkv, a.hd, a.max_rows, a.max_len, a.prefix_len);
   if (workspace_bytes < p.o_bytes + p.ml_bytes || (p.parts > 0 && !workspace)) return PE_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 15) return PE_ERR_ARG;
+  // rows and work units are counted in 32 bits
+  if (a.M * a.nh >= (int64_t(1) << 31) || p.units >= (int64_t(1) << 31) ||
+      (int64_t)a.batch * a.nkv * p.nsplit * p.seq.blocks >= (int64_t(1) << 31))
+    return PE_ERR_ARG;
   p.pt.o = (float*)workspace;
   p.pt.ml = (float*)((char*)workspace + p.o_bytes);
   const bool mod = a.softcap > 0.f || a.slopes || a.window > 0;
