@@ -11,9 +11,10 @@
 // cores (and the exponentials beside them) where a per-sequence pass would read
 // it once per sequence. A sequence's own keys serve its own rows only.
 //
-// Two launches: the prefix's parts, then the sequences' own keys, whose
-// workgroups join the prefix's parts to theirs and write the output. A third
-// launch joins the parts where a sequence's own keys are split as well.
+// The prefix's and the sequences' own keys are shares of one launch, whose parts
+// a second one joins; a large prefix (many rows over many keys) gets a launch of
+// its own with wider row blocks first, and the sequences' workgroups join its
+// parts to theirs and write the output themselves.
 //
 // Products as in the contiguous kernels: S^T = K Q^T (A = 32 keys, B = the
 // wave's 32 rows, held in registers), so that a lane owns one row and 16 of 32
@@ -68,12 +69,12 @@ __device__ __forceinline__ void wait_vm() {
 // One list of pages as the key source of a KV head.
 struct Pages {
   const int32_t* table;
-  int64_t lo, hi;  // keys read: [lo, hi), the others of a step as the nearest of them
+  int lo, hi;  // keys read (counted in 32 bits: a sequence is shorter than 2^30), [lo, hi), the others of a step as the nearest
 };
 
 // What a lane's row needs besides its Q.
 struct RowInfo {
-  int64_t node;   // causal: its token's index among the sequence's new rows; tree: unused
+  int node;       // causal: its token's index among the sequence's new rows; tree: unused
   int rel;        // its position - the position of key 0 of the list (MOD)
   float slope2;   // slope * log2 e (MOD)
   int lo, tile_lo;  // first cached key its window holds; the largest of the tile's (MOD)
@@ -81,12 +82,16 @@ struct RowInfo {
 };
 static_assert(PE_TREE_MAX_WORDS == 4, "one field per word");
 
-// The configuration of a workgroup: W waves of one 32-row tile each, SB 32-key
-// blocks in a step, a ring of ST steps in LDS filled straight from global memory
-// (ST - 1 of them in flight while one is multiplied).
-template <int HD_, int W_, int SB_, int ST_>
+// The configuration of a workgroup: W waves, DS of them on one 32-row tile (each
+// forms the tile's scores and keeps hd / DS dims of its O; with few tiles a
+// workgroup waits for keys, and this needs no exchange between its waves), SB
+// 32-key blocks in a step, a ring of ST steps in LDS filled straight from global
+// memory (ST - 1 of them in flight while one is multiplied).
+template <int HD_, int W_, int DS_, int SB_, int ST_>
 struct Cfg {
-  static constexpr int HD = HD_, W = W_, SB = SB_, ST = ST_;
+  static constexpr int HD = HD_, W = W_, DS = DS_, SB = SB_, ST = ST_;
+  static constexpr int NT = W / DS;                     // row tiles
+  static constexpr int OB = HD / 32 / DS;               // 32-dim blocks of O a wave holds
   static constexpr int SK = 32 * SB;                    // keys of a step
   static constexpr int kHalf = SK * HD * 2;             // bytes of a step's K (and of its V)
   static constexpr int kStep = 2 * kHalf;
@@ -99,20 +104,21 @@ struct Cfg {
 
 // One 64-bit-masked step's visibility, bit j: key kb0 + j. Tree rows see keys
 // below P and the nodes of their bits; causal rows those up to P + node.
-__device__ __forceinline__ uint64_t node_window(int64_t kb0, int64_t P, const RowInfo& r) {
-  const int64_t off = kb0 - P;  // node index of key kb0
+__device__ __forceinline__ uint64_t node_window(int kb0, int P, uint64_t n0, uint64_t n1, uint64_t n2,
+                                                uint64_t n3) {
+  const int off = kb0 - P;  // node index of key kb0
   if (off <= -64) return ~0ull;
   if (off < 0) {
-    const int j0 = (int)(-off);
-    return ((1ull << j0) - 1) | (r.nb0 << j0);
+    const int j0 = -off;
+    return ((1ull << j0) - 1) | (n0 << j0);
   }
   if (off >= 64 * PE_TREE_MAX_WORDS) return 0ull;
-  const int wi = (int)(off >> 6), sh = (int)(off & 63);
-  const uint64_t a = wi == 0 ? r.nb0 : wi == 1 ? r.nb1 : wi == 2 ? r.nb2 : r.nb3;
-  const uint64_t b = wi == 0 ? r.nb1 : wi == 1 ? r.nb2 : wi == 2 ? r.nb3 : 0ull;
+  const int wi = off >> 6, sh = off & 63;
+  const uint64_t a = wi == 0 ? n0 : wi == 1 ? n1 : wi == 2 ? n2 : n3;
+  const uint64_t b = wi == 0 ? n1 : wi == 1 ? n2 : wi == 2 ? n3 : 0ull;
   return sh ? (a >> sh) | (b << (64 - sh)) : a;
 }
-__device__ __forceinline__ uint64_t below(int64_t n) {  // bits 0 .. n - 1
+__device__ __forceinline__ uint64_t below(int n) {  // bits 0 .. n - 1
   return n >= 64 ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1);
 }
 
@@ -123,22 +129,22 @@ __device__ __forceinline__ uint64_t below(int64_t n) {  // bits 0 .. n - 1
 // to key 0 (MOD, where distances count).
 template <int DT, typename C, bool MOD, bool PRE>
 __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const Pages& pg, int kvh, int s0, int s1,
-                                       int64_t P, int new_rows, bool live, int64_t last_key, const RowInfo& ri,
+                                       int P, int new_rows, bool live, int last_key, RowInfo ri,
                                        const u32x4_t (&qf)[C::HD / 16], const int* npos, bool& bad,
-                                       f32x16_t (&o)[C::HD / 32], float& m, float& l) {
-  constexpr int HD = C::HD, SB = C::SB;
+                                       f32x16_t (&o)[C::OB], float& m, float& l) {
+  constexpr int HD = C::HD, SB = C::SB, OB = C::OB;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int ln = lane & 31, g = lane >> 5;
+  const int ln = lane & 31, g = lane >> 5, hb = (wave % C::DS) * OB;
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
   typedef const __attribute__((address_space(4))) int32_t* const_i32;  // read through the scalar cache
   const const_i32 tab = (const_i32)(uintptr_t)uniform_ptr((const uint16_t*)pg.table);
   const int psl = a.ps_log2;
-  const int64_t clo = pg.lo >> 4, chi = (pg.hi - 1) >> 4;
+  const int clo = pg.lo >> 4, chi = (pg.hi - 1) >> 4;
   // the pages of this wave's pieces of a step, asked for a step ahead
   int page[C::kChunks];
   auto piece_of = [&](int step, int c) {
     const int ch = (wave * C::kChunks + c) % (C::SK / 16);
-    const int64_t k = (int64_t)step * (C::SK / 16) + ch;
+    const int k = step * (C::SK / 16) + ch;
     return k < clo ? clo : k > chi ? chi : k;
   };
   auto ask = [&](int step) {
@@ -151,7 +157,7 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
     for (int c = 0; c < C::kChunks; ++c) {
       const int piece = wave * C::kChunks + c, ch = piece % (C::SK / 16);
       const bool is_v = piece >= C::SK / 16;
-      const int64_t k16 = piece_of(step, c);
+      const int k16 = piece_of(step, c);
       int pgid = page[c];
       if (pgid < 0 || pgid >= a.num_pages) {
         bad = true;
@@ -161,7 +167,7 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
       const uint16_t* src = uniform_ptr((const uint16_t*)(is_v ? a.v_pool : a.k_pool) + row * HD);
       const uint32_t dst =
           __builtin_amdgcn_readfirstlane(buf + (is_v ? C::kHalf : 0) + ch * 16 * HD * 2);
-      const int rlo = (int)max(pg.lo - (k16 << 4), (int64_t)0), rhi = (int)min(pg.hi - 1 - (k16 << 4), (int64_t)15);
+      const int rlo = max(pg.lo - (k16 << 4), 0), rhi = min(pg.hi - 1 - (k16 << 4), 15);
 #pragma unroll
       for (int i = 0; i < C::kPerChunk; ++i) {
         constexpr int kLanes = HD / 8;  // lanes on a row
@@ -173,7 +179,7 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
   };
 
 #pragma unroll
-  for (int h = 0; h < HD / 32; ++h)
+  for (int h = 0; h < OB; ++h)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[h][i] = 0.f;
   m = kPagedInitMax;
@@ -201,7 +207,7 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
       issue(s + C::ST - 1);
       if (s + C::ST < s1) ask(s + C::ST);
     }
-    const int64_t kb0 = (int64_t)s * C::SK;
+    const int kb0 = s * C::SK;
     if (!live || kb0 > last_key) continue;  // wave-uniform: the tile sees no key of this step
     const uint8_t* kbp = smem + (s % C::ST) * C::kStep;
     const uint8_t* vbp = kbp + C::kHalf;
@@ -234,14 +240,14 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
 #pragma unroll
           for (int i = 0; i < 16; ++i) sc[sb][i] *= scale2;
       }
-      const int d0 = ri.rel - (int)kb0 - 4 * g;  // distance of key kb0 + 4 g
+      const int d0 = ri.rel - kb0 - 4 * g;  // distance of key kb0 + 4 g
       if (node_step && tree && npos) {  // new rows lie where their positions say
 #pragma unroll
         for (int sb = 0; sb < SB; ++sb)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int off = 32 * sb + 8 * (i >> 2) + (i & 3);
-            const int u = (int)(kb0 - P) + off + 4 * g;
+            const int u = kb0 - P + off + 4 * g;
             const int np = npos[max(0, min(u, new_rows - 1))];
             const int dist = u < 0 ? d0 - off : ri.rel - np;
             sc[sb][i] = fmaf(-ri.slope2, (float)dist, sc[sb][i]);
@@ -259,9 +265,9 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
     if constexpr (MOD) edge = edge || kb0 < ri.tile_lo;
     if (edge) {
       uint64_t win = ~0ull;
-      if constexpr (!PRE) win = tree ? node_window(kb0, P, ri) : below(P + ri.node + 1 - kb0);
-      int64_t lo = pg.lo;
-      if constexpr (MOD) lo = max(lo, (int64_t)ri.lo);
+      if constexpr (!PRE) win = tree ? node_window(kb0, P, ri.nb0, ri.nb1, ri.nb2, ri.nb3) : below(P + ri.node + 1 - kb0);
+      int lo = pg.lo;
+      if constexpr (MOD) lo = max(lo, ri.lo);
       win &= below(pg.hi - kb0) & ~below(lo - kb0);
       win >>= 4 * g;
 #pragma unroll
@@ -294,7 +300,7 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
     l = l * alpha + psum;
     if (__builtin_amdgcn_ballot_w64(mnew != m) != 0ull) {
 #pragma unroll
-      for (int h = 0; h < HD / 32; ++h)
+      for (int h = 0; h < OB; ++h)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[h][i] *= alpha;
     }
@@ -307,8 +313,8 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
       const u32x4_t bp = {pb[sb][4 * cq], pb[sb][4 * cq + 1], pb[sb][4 * cq + 2], pb[sb][4 * cq + 3]};
       const int kb = 16 * c + 4 * (qg >> 1) + (jl >> 2);
 #pragma unroll
-      for (int h = 0; h < HD / 32; ++h) {
-        const int db = 32 * h + 16 * (qg & 1) + 4 * (jl & 3);
+      for (int h = 0; h < OB; ++h) {
+        const int db = 32 * (hb + h) + 16 * (qg & 1) + 4 * (jl & 3);
         typedef short s4v_t __attribute__((__vector_size__(4 * sizeof(short))));
         typedef __attribute__((address_space(3))) s4v_t lds_s4v_t;
         const uint2 lo = __builtin_bit_cast(
@@ -334,16 +340,17 @@ __device__ __forceinline__ int64_t part_tile(const PagedParts& p, int nkv, int p
   return (((int64_t)part * nkv + kvh) * p.tiles + tile) * (32 * HD);
 }
 
-template <int HD>
-__device__ __forceinline__ void store_part(const PagedParts& p, int nkv, int part, int kvh, uint32_t row, int g,
-                                           const f32x16_t (&o)[HD / 32], float m, float l) {
-  float* dst = p.o + part_tile<HD>(p, nkv, part, kvh, row >> 5) + ((row & 31) + 32 * g) * 4;
+// `hb`: the first 32-dim block of O held.
+template <int HD, int OB>
+__device__ __forceinline__ void store_part(const PagedParts& p, int nkv, int part, int kvh, uint32_t row, int g, int hb,
+                                           const f32x16_t (&o)[OB], float m, float l) {
+  float* dst = p.o + part_tile<HD>(p, nkv, part, kvh, row >> 5) + ((row & 31) + 32 * g) * 4 + hb * 1024;
 #pragma unroll
-  for (int h = 0; h < HD / 32; ++h)
+  for (int h = 0; h < OB; ++h)
 #pragma unroll
     for (int c = 0; c < 4; ++c)
       *(f32x4_t*)(dst + (4 * h + c) * 256) = f32x4_t{o[h][4 * c], o[h][4 * c + 1], o[h][4 * c + 2], o[h][4 * c + 3]};
-  if (g == 0) {
+  if (g == 0 && hb == 0) {
     float2* ml = (float2*)p.ml + ((int64_t)part * nkv + kvh) * p.tiles * 32 + row;
     *ml = make_float2(m, l);
   }
@@ -374,17 +381,15 @@ __device__ __forceinline__ int window_lo(const PagedAttn& a, RowInfo& ri, int ca
 }
 
 // ---------------------------------------------------------------------------
-// The prefix
+// The prefix: workgroup `w`'s share of the row blocks' key steps
 // ---------------------------------------------------------------------------
 template <int DT, typename C, bool MOD>
-__global__ __launch_bounds__(64 * C::W, 2) void paged_prefix_kernel(PagedAttn a, PagedPrefix pp, PagedParts parts) {
+__device__ __forceinline__ void prefix_share(const PagedAttn& a, const PagedPrefix& pp, const PagedParts& parts,
+                                             uint32_t w, uint8_t* smem, int* s_lo) {
   constexpr int HD = C::HD;
-  __shared__ __align__(1024) uint8_t smem[C::kSmem];
-  __shared__ int s_lo[C::W];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int ln = lane & 31, g = lane >> 5, tile = wave;
+  const int ln = lane & 31, g = lane >> 5, tile = wave / C::DS, hb = (wave % C::DS) * C::OB;
   const uint32_t G = (uint32_t)(a.nh / a.nkv), R = (uint32_t)a.M * G;
-  const uint32_t w = xcd_item(blockIdx.x, gridDim.x);
   const uint32_t uend = min(pp.total, (w + 1) * pp.per);
   bool bad = false;
   for (uint32_t u = w * pp.per; u < uend;) {
@@ -402,39 +407,46 @@ __global__ __launch_bounds__(64 * C::W, 2) void paged_prefix_kernel(PagedAttn a,
 #pragma unroll
     for (int j = 0; j < HD / 16; ++j) qf[j] = *(const u32x4_t*)(qr + 16 * j);
     RowInfo ri;
-    Pages pg{a.prefix_table, 0, a.prefix_len};
+    const int S0 = (int)a.prefix_len;
+    Pages pg{a.prefix_table, 0, S0};
     int first = s0;
     if constexpr (MOD) {
       ri.rel = a.positions ? (int)a.positions[tok] : 0;
       ri.slope2 = a.slopes ? a.slopes[hq] * kLog2e : 0.f;
-      const int lo = window_lo<C::W>(a, ri, (int)a.prefix_len, live, s_lo);
-      pg.lo = min((int64_t)lo, a.prefix_len - 1);
-      if (lo > 0) first = lo >= a.prefix_len ? s1 : max(s0, lo / C::SK);  // steps behind every row's window
+      const int lo = window_lo<C::W>(a, ri, S0, live, s_lo);
+      pg.lo = min(lo, S0 - 1);
+      if (lo > 0) first = lo >= S0 ? s1 : max(s0, lo / C::SK);  // steps behind every row's window
     }
-    f32x16_t o[HD / 32];
+    f32x16_t o[C::OB];
     float m, l;
-    attend<DT, C, MOD, true>(a, smem, pg, kvh, first, max(first, s1), a.prefix_len, 0, live, a.prefix_len - 1, ri, qf,
-                             nullptr, bad, o, m, l);
+    attend<DT, C, MOD, true>(a, smem, pg, kvh, first, max(first, s1), S0, 0, live, S0 - 1, ri, qf, nullptr, bad, o, m, l);
     if (live)
-      store_part<HD>(parts, a.nkv, (int)(w - prefix_first_wg(pp, x)), kvh, row0 + ln, g, o, m, l);
+      store_part<HD, C::OB>(parts, a.nkv, (int)(w - prefix_first_wg(pp, x)), kvh, row0 + ln, g, hb, o, m, l);
   }
   if (bad && lane == 0) atomicOr(a.status, PE_ERR_INDEX);
 }
 
 // ---------------------------------------------------------------------------
-// The sequences' own keys
+// The sequences' own keys: item = (key split of kps keys, sequence, KV head,
+// block of row tiles)
 // ---------------------------------------------------------------------------
-// Workgroup = (sequence, KV head, key split of kps keys, block of NT row tiles).
-// A sequence of one split joins the prefix's parts of its rows to its own and
-// writes the output; otherwise each split is a part and paged_join_kernel does.
-template <int DT, int HD>
-__device__ __forceinline__ void write_out(const PagedAttn& a, int64_t tok, int hq, int g, const f32x16_t (&o)[HD / 32],
+// The launch's shares of it. `direct`: a sequence of one split joins the
+// prefix's parts of its rows to its own (an earlier launch wrote them, and they
+// are few) and writes the output; otherwise its result is a part as well and
+// paged_join_kernel writes the output.
+struct PagedSeqs {
+  uint32_t items, kps, nblk, block_rows;
+  int nsplit, kind, direct;
+};
+
+template <int DT, int OB>
+__device__ __forceinline__ void write_out(const PagedAttn& a, int64_t tok, int64_t col, const f32x16_t (&o)[OB],
                                           float l) {
   typedef typename Elem<DT>::T Te;
-  Te* dst = (Te*)a.out + tok * a.ld_out + (int64_t)hq * HD + 4 * g;
+  Te* dst = (Te*)a.out + tok * a.ld_out + col;
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int h = 0; h < HD / 32; ++h)
+  for (int h = 0; h < OB; ++h)
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const float v[4] = {o[h][4 * c] * inv, o[h][4 * c + 1] * inv, o[h][4 * c + 2] * inv, o[h][4 * c + 3] * inv};
@@ -443,21 +455,16 @@ __device__ __forceinline__ void write_out(const PagedAttn& a, int64_t tok, int h
 }
 
 template <int DT, typename C, bool MOD>
-__global__ __launch_bounds__(64 * C::W, 2) void paged_seq_kernel(PagedAttn a, PagedPrefix pp, PagedParts parts,
-                                                                 uint32_t kps, int nsplit, int nblk,
-                                                                 uint32_t block_rows) {
+__device__ __forceinline__ void seq_item(const PagedAttn& a, const PagedPrefix& pp, const PagedParts& parts,
+                                         const PagedSeqs& sq, uint32_t item, uint8_t* smem, int* s_npos, int* s_lo) {
   constexpr int HD = C::HD;
-  __shared__ __align__(1024) uint8_t smem[C::kSmem];
-  __shared__ int s_npos[MOD ? 64 * PE_TREE_MAX_WORDS : 1];
-  __shared__ int s_lo[C::W];
   // blocks of one (split, sequence, KV head) on one XCD, neighbours in time;
   // otherwise KV heads over the XCDs (workgroup i starts on XCD i % 8), so that
   // sequences of different lengths load them alike, and the last splits, which
   // short sequences leave empty, at the end
-  const uint32_t n1 = gridDim.x / (uint32_t)nblk;
-  uint32_t item = blockIdx.x, blk = 0;
-  if (nblk > 1) {
-    const uint32_t per = n1 & 7 ? 1 : 8, q = item / (per * nblk), r = item - q * per * nblk;
+  uint32_t blk = 0;
+  if (sq.nblk > 1) {
+    const uint32_t per = sq.items / sq.nblk & 7 ? 1 : 8, q = item / (per * sq.nblk), r = item - q * per * sq.nblk;
     blk = r / per;
     item = q * per + (r - blk * per);
   }
@@ -471,13 +478,13 @@ __global__ __launch_bounds__(64 * C::W, 2) void paged_seq_kernel(PagedAttn a, Pa
   }
   const int T = s.rows;
   const uint32_t G = (uint32_t)(a.nh / a.nkv), R = T * G;
-  const int64_t P = s.priv, S = P + T;
-  const uint32_t blk0 = blk * block_rows;
-  const int my_splits = (int)(((uint32_t)S + kps - 1) / kps);
+  const int P = (int)s.priv, S = P + T;
+  const uint32_t blk0 = blk * sq.block_rows;
+  const int my_splits = (int)(((uint32_t)S + sq.kps - 1) / sq.kps);
   if (blk0 >= R || split >= my_splits) return;
-  const int ln = lane & 31, g = lane >> 5, tile = wave;
+  const int ln = lane & 31, g = lane >> 5, tile = wave / C::DS, hb = (wave % C::DS) * C::OB;
   const bool tree = a.mask_mode == PE_MASK_TREE;
-  const uint32_t row0 = blk0 + 32 * tile, row_end = min(blk0 + block_rows, R);
+  const uint32_t row0 = blk0 + 32 * tile, row_end = min(blk0 + sq.block_rows, R);
   const bool live = row0 < row_end;
   const uint32_t row = min(row0 + ln, R - 1);
   const int t = (int)(row / G);
@@ -498,30 +505,29 @@ __global__ __launch_bounds__(64 * C::W, 2) void paged_seq_kernel(PagedAttn a, Pa
     if (a.words > 3) ri.nb3 = bt[3];
   }
   // the keys some row of the block sees end at hi; of this wave's tile, at last_key
-  const int t_blk = min(T - 1, (int)((blk0 + block_rows - 1) / G));
+  const int t_blk = min(T - 1, (int)((blk0 + sq.block_rows - 1) / G));
   const int t_tile = min(T - 1, (int)((row0 + 31) / G));
   Pages pg{a.block_table + b * a.ld_table, 0, tree ? S : P + t_blk + 1};
-  const int64_t last_key = tree ? S - 1 : P + t_tile;
+  const int last_key = tree ? S - 1 : P + t_tile;
   if constexpr (MOD) {
     ri.rel = a.positions ? (int)(a.positions[tok] - a.prefix_len) : 0;
     ri.slope2 = a.slopes ? a.slopes[hq] * kLog2e : 0.f;
     if (a.positions && tree)
       for (int u = tid; u < T; u += 64 * C::W) s_npos[u] = (int)(a.positions[s.row0 + u] - a.prefix_len);
-    pg.lo = window_lo<C::W>(a, ri, (int)(tree ? P : pg.hi - 1), live, s_lo);
+    pg.lo = window_lo<C::W>(a, ri, tree ? P : pg.hi - 1, live, s_lo);
   }
-  const int64_t k0 = (int64_t)split * kps, k1 = min(pg.hi, k0 + (int64_t)kps);
-  const int s1 = (int)((k1 + C::SK - 1) / C::SK);
-  const int s0 = (int)max(k0 / C::SK, pg.lo / C::SK);
+  const int k0 = split * (int)sq.kps, k1 = min(pg.hi, k0 + (int)sq.kps);
+  const int s1 = (k1 + C::SK - 1) / C::SK, s0 = max(k0, pg.lo) / C::SK;
   bool bad = false;
-  f32x16_t o[HD / 32];
+  f32x16_t o[C::OB];
   float m, l;
   attend<DT, C, MOD, false>(a, smem, pg, kvh, s0, max(s0, s1), P, T, live, last_key, ri, qf,
                             MOD && a.positions ? s_npos : nullptr, bad, o, m, l);
   if (bad && lane == 0) atomicOr(a.status, PE_ERR_INDEX);
   if (row0 + ln >= row_end) return;
   const uint32_t grow = (uint32_t)s.row0 * G + row;  // the row among the whole batch's
-  if (my_splits > 1) {
-    store_part<HD>(parts, a.nkv, parts.pre_parts + split, kvh, grow, g, o, m, l);
+  if (my_splits > 1 || !sq.direct) {
+    store_part<HD, C::OB>(parts, a.nkv, parts.pre_parts + split, kvh, grow, g, hb, o, m, l);
     return;
   }
   if (parts.pre_parts > 0) {
@@ -532,9 +538,9 @@ __global__ __launch_bounds__(64 * C::W, 2) void paged_seq_kernel(PagedAttn a, Pa
       const float a0 = __builtin_amdgcn_exp2f(m - mx), a1 = __builtin_amdgcn_exp2f(ml.x - mx);
       m = mx;
       l = a0 * l + a1 * ml.y;
-      const float* src = parts.o + part_tile<HD>(parts, a.nkv, p, kvh, grow >> 5) + ((grow & 31) + 32 * g) * 4;
+      const float* src = parts.o + part_tile<HD>(parts, a.nkv, p, kvh, grow >> 5) + ((grow & 31) + 32 * g) * 4 + hb * 1024;
 #pragma unroll
-      for (int h = 0; h < HD / 32; ++h)
+      for (int h = 0; h < C::OB; ++h)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const f32x4_t o1 = *(const f32x4_t*)(src + (4 * h + c) * 256);
@@ -543,25 +549,70 @@ __global__ __launch_bounds__(64 * C::W, 2) void paged_seq_kernel(PagedAttn a, Pa
         }
     }
   }
-  write_out<DT, HD>(a, tok, hq, g, o, l);
+  write_out<DT, C::OB>(a, tok, (int64_t)hq * HD + 32 * hb + 4 * g, o, l);
 }
 
-// Joins the parts of the sequences whose own keys are split: one thread per
-// (row, four dims), the prefix's parts first, then the splits in key order.
+// ---------------------------------------------------------------------------
+// Kernels
+// ---------------------------------------------------------------------------
+// Many rows over a long prefix: eight tiles (256 rows) on every K / V byte, one
+// workgroup per CU.
+template <int HD> using Wide = Cfg<HD, 8, 1, 2, 4>;
+// Four waves, 64 KiB of LDS (32 KiB for heads of 64), two workgroups per CU.
+template <int HD> using Four = Cfg<HD, 4, 1, 2, 2>;
+template <int HD> using Two = Cfg<HD, 4, 2, HD == 128 ? 1 : 2, 4>;
+template <int HD> using One = Cfg<HD, 4, HD == 128 ? 4 : 2, HD == 128 ? 1 : 2, 4>;
+
+template <int DT, int HD, bool MOD>
+__global__ __launch_bounds__(512, 2) void paged_prefix_kernel(PagedAttn a, PagedPrefix pp, PagedParts parts) {
+  __shared__ __align__(1024) uint8_t smem[Wide<HD>::kSmem];
+  __shared__ int s_lo[8];
+  prefix_share<DT, Wide<HD>, MOD>(a, pp, parts, xcd_item(blockIdx.x, gridDim.x), smem, s_lo);
+}
+
+// Workgroups [0, n_pre) take the prefix, the rest the sequences' own keys: on
+// the two places of a CU the one waits for the matrix cores while the other
+// waits for memory.
+template <int DT, int HD, bool MOD>
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttn a, PagedPrefix pp, PagedParts parts, PagedSeqs sq,
+                                                            uint32_t n_pre, int pre_kind) {
+  constexpr int kSmem = Two<HD>::kSmem > Four<HD>::kSmem ? Two<HD>::kSmem : Four<HD>::kSmem;
+  static_assert(One<HD>::kSmem <= kSmem, "one ring for every kind");
+  __shared__ __align__(1024) uint8_t smem[kSmem];
+  __shared__ int s_npos[MOD ? 64 * PE_TREE_MAX_WORDS : 1];
+  __shared__ int s_lo[4];
+  if (blockIdx.x < n_pre) {
+    const uint32_t w = xcd_item(blockIdx.x, n_pre);
+    if (pre_kind == 4) prefix_share<DT, Four<HD>, MOD>(a, pp, parts, w, smem, s_lo);
+    else if (pre_kind == 2) prefix_share<DT, Two<HD>, MOD>(a, pp, parts, w, smem, s_lo);
+    else prefix_share<DT, One<HD>, MOD>(a, pp, parts, w, smem, s_lo);
+  } else {
+    const uint32_t item = blockIdx.x - n_pre;
+    if (sq.kind == 4) seq_item<DT, Four<HD>, MOD>(a, pp, parts, sq, item, smem, s_npos, s_lo);
+    else if (sq.kind == 2) seq_item<DT, Two<HD>, MOD>(a, pp, parts, sq, item, smem, s_npos, s_lo);
+    else seq_item<DT, One<HD>, MOD>(a, pp, parts, sq, item, smem, s_npos, s_lo);
+  }
+}
+
+// Joins the parts: one thread per (row, four dims), 32 rows x 32 dims a block
+// (512 contiguous bytes of a part per load), the prefix's parts first, then the
+// splits in key order.
 template <int DT, int HD>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefix pp, PagedParts parts, uint32_t kps) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefix pp, PagedParts parts, PagedSeqs sq) {
   const int b = blockIdx.z, kvh = blockIdx.y;
   const PagedSeq s = paged_seq(a, b);
   if (!s.ok) return;
-  const int my_splits = (int)(((uint32_t)(s.priv + s.rows) + kps - 1) / kps);
+  const int my_splits = (int)(((uint32_t)(s.priv + s.rows) + sq.kps - 1) / sq.kps);
   const uint32_t G = (uint32_t)(a.nh / a.nkv), R = s.rows * G;
-  // thread order inside a block: rows fastest, as a part's tile is stored
-  const uint32_t row = blockIdx.x * (1024 / HD) + threadIdx.x % (1024 / HD);
-  const int piece = threadIdx.x / (1024 / HD);  // dims 4 piece .. + 3
-  if (my_splits <= 1 || row >= R) return;
+  const uint32_t row = blockIdx.x / (HD / 32) * 32 + (threadIdx.x & 31);
+  const int piece = (int)(blockIdx.x % (HD / 32)) * 8 + (int)(threadIdx.x >> 5);  // dims 4 piece .. + 3
+  if ((my_splits <= 1 && sq.direct) || row >= R) return;
   const uint32_t grow = (uint32_t)s.row0 * G + row;
   const int npre = parts.pre_parts > 0 ? prefix_parts_of(pp, kvh * pp.nblk + grow / pp.block_rows) : 0;
-  const int at = (piece >> 1) * 256 + ((int)(grow & 31) + 32 * (piece & 1)) * 4;
+  const float* src = parts.o + part_tile<HD>(parts, a.nkv, 0, kvh, grow >> 5) + (piece >> 1) * 256 +
+                     ((int)(grow & 31) + 32 * (piece & 1)) * 4;
+  const float2* sml = (const float2*)parts.ml + (int64_t)kvh * parts.tiles * 32 + grow;
+  const int64_t o_part = (int64_t)a.nkv * parts.tiles * (32 * HD), ml_part = (int64_t)a.nkv * parts.tiles * 32;
   float m = kPagedInitMax, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   constexpr int kAhead = 4;  // parts asked for before the first is joined
   const int n = npre + my_splits;
@@ -571,8 +622,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefi
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int i = min(i0 + k, n - 1), p = i < npre ? i : parts.pre_parts + i - npre;
-      ml[k] = ((const float2*)parts.ml)[((int64_t)p * a.nkv + kvh) * parts.tiles * 32 + grow];
-      v[k] = *(const f32x4_t*)(parts.o + part_tile<HD>(parts, a.nkv, p, kvh, grow >> 5) + at);
+      ml[k] = sml[p * ml_part];
+      v[k] = *(const f32x4_t*)(src + p * o_part);
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
@@ -595,28 +646,30 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefi
 
 // ------------------------------------------------------------------ plans
 constexpr int kCus = 256;
-constexpr int kSeqWgs = 2048, kMinSplit = 256, kSplitRows = 8, kPrefixSteps = 4;
+constexpr int kSeqWgs = 2048, kMinSplit = 256, kSplitRows = 8, kPrefixSteps = 4, kFusedPre = 256;
+constexpr int64_t kWideUnits = 4096;
 
 // A launch's workgroups: which configuration, row tiles per block and how many
 // blocks hold `tiles` row tiles in equal shares.
 struct Shape {
-  int kind, tiles, blocks;
+  int kind, tiles;
+  int64_t blocks;
 };
-Shape shape_of(int64_t tiles) {
-  const int most = tiles > 4 ? 8 : tiles > 2 ? 4 : (int)tiles;
+Shape shape_of(int64_t tiles, int most) {
   const int64_t blocks = (tiles + most - 1) / most;
-  return {most == 8 ? 0 : most == 4 ? 1 : most == 2 ? 2 : 3, (int)((tiles + blocks - 1) / blocks), (int)blocks};
+  const int each = (int)((tiles + blocks - 1) / blocks);
+  return {most == 8 ? 8 : each > 2 ? 4 : each, each, blocks};
 }
-// Keys of a step: 64, but 32 for 128-dim heads with at most four tiles.
-int step_keys(const Shape& s, int hd) { return s.kind == 0 || hd == 64 ? 64 : 32; }
+// Keys of a step: 32 for 128-dim heads with one or two tiles, else 64.
+int step_keys(const Shape& s, int hd) { return hd == 64 || s.kind >= 4 ? 64 : 32; }
 
 struct Plan {
   PagedPrefix pp;
-  Shape pre, seq;
-  int64_t units, pre_wgs, o_bytes, ml_bytes;
-  uint32_t kps;
-  int nsplit, parts;
+  PagedSeqs sq;
   PagedParts pt;
+  bool wide, join;
+  int pre_kind;
+  int64_t units, items, pre_wgs, o_bytes, ml_bytes;
 };
 
 Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int64_t max_len, int64_t prefix_len) {
@@ -625,74 +678,54 @@ Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int6
   const int64_t tiles = (M * G + 31) / 32;
   p.pt.tiles = tiles;
   p.pp = PagedPrefix{0, 1, 1, 1, 32};
-  p.pre = Shape{0, 8, 1};
   p.pre_wgs = p.units = 0;
-  p.pt.pre_parts = 0;
+  p.pt.pre_parts = p.pre_kind = 0;
+  p.wide = false;
   if (prefix_len > 0) {
-    p.pre = shape_of(tiles);
-    const int64_t steps = (prefix_len - 1) / step_keys(p.pre, hd) + 1;
-    const int64_t total = (int64_t)nkv * p.pre.blocks * steps;
-    p.units = total;
-    const int64_t room = kCus * (p.pre.kind == 0 ? 1 : 2);
-    const int64_t blocks = (int64_t)nkv * p.pre.blocks;
-    const int64_t want = std::min<int64_t>(room, std::max(blocks, total / kPrefixSteps));
-    p.pp = PagedPrefix{(uint32_t)total, (uint32_t)((total + want - 1) / want), (uint32_t)steps, (uint32_t)p.pre.blocks,
-                       (uint32_t)(32 * p.pre.tiles)};
-    p.pre_wgs = (total + p.pp.per - 1) / p.pp.per;
-    p.pt.pre_parts = (int)((steps - 1) / p.pp.per) + 2;
+    const int64_t s64 = (prefix_len - 1) / 64 + 1;
+    // many rows over many keys: the wide blocks' own launch
+    p.wide = tiles > 4 && tiles * s64 * nkv >= kWideUnits * 8;
+    const Shape pre = shape_of(tiles, p.wide ? 8 : 4);
+    p.pre_kind = pre.kind;
+    const int64_t steps = (prefix_len - 1) / step_keys(pre, hd) + 1, blocks = nkv * pre.blocks;
+    p.units = blocks * steps;
+    const int64_t want = std::min<int64_t>(p.wide ? kCus : kFusedPre, std::max(blocks, p.units / kPrefixSteps));
+    const int64_t per = (p.units + want - 1) / want;
+    p.pp = PagedPrefix{(uint32_t)p.units, (uint32_t)per, (uint32_t)steps, (uint32_t)pre.blocks, (uint32_t)(32 * pre.tiles)};
+    p.pre_wgs = (p.units + per - 1) / per;
+    p.pt.pre_parts = (int)((steps - 1) / per) + 2;
   }
-  p.seq = shape_of(((int64_t)max_rows * G + 31) / 32);
+  const Shape seq = shape_of(((int64_t)max_rows * G + 31) / 32, 4);
   const int64_t keys = max_len - prefix_len + max_rows;
-  const int64_t wgs = (int64_t)batch * nkv * p.seq.blocks;
-  const int64_t least = std::max<int64_t>(kMinSplit, kSplitRows * max_rows * G);
-  const int64_t ns = std::max<int64_t>(1, std::min<int64_t>(kSeqWgs / wgs, keys / least));
-  p.kps = (uint32_t)((((keys + ns - 1) / ns + 63) / 64) * 64);
-  p.nsplit = (int)((keys + p.kps - 1) / p.kps);
-  p.parts = p.pt.pre_parts + (p.nsplit > 1 ? p.nsplit : 0);
-  p.o_bytes = (int64_t)p.parts * nkv * p.pt.tiles * 32 * hd * 4;
-  p.ml_bytes = (int64_t)p.parts * nkv * p.pt.tiles * 32 * 8;
+  const int64_t wgs = batch * nkv * seq.blocks;
+  const int64_t least = std::max<int64_t>(kMinSplit, kSplitRows * std::min<int64_t>(32 * seq.tiles, max_rows * G));
+  int64_t ns = std::max(std::min<int64_t>(2 * kCus / wgs, keys / kMinSplit), std::min<int64_t>(kSeqWgs / wgs, keys / least));
+  ns = std::max<int64_t>(1, ns);
+  const int64_t kps = (((keys + ns - 1) / ns + 63) / 64) * 64;
+  const int64_t nsplit = (keys + kps - 1) / kps;
+  p.items = wgs * nsplit;
+  const bool direct = prefix_len == 0 || (p.wide && p.pt.pre_parts <= 3);
+  p.sq = PagedSeqs{(uint32_t)p.items, (uint32_t)kps, (uint32_t)seq.blocks, (uint32_t)(32 * seq.tiles), (int)nsplit, seq.kind,
+                   direct};
+  p.join = nsplit > 1 || !direct;
+  const int64_t parts = p.pt.pre_parts + (p.join ? nsplit : 0);
+  p.o_bytes = parts * nkv * tiles * 32 * hd * 4;
+  p.ml_bytes = parts * nkv * tiles * 32 * 8;
   return p;
-}
-
-template <int HD> using Wide = Cfg<HD, 8, 2, 4>;
-template <int HD, int W> using Slim = Cfg<HD, W, HD == 128 ? 1 : 2, 3>;
-#define PE_ARG(...) __VA_ARGS__
-
-template <int DT, int HD, bool MOD>
-void launch_prefix(const Plan& p, const PagedAttn& a, hipStream_t st) {
-  const unsigned n = (unsigned)p.pre_wgs;
-  switch (p.pre.kind) {
-    case 0: paged_prefix_kernel<DT, Wide<HD>, MOD><<<n, 512, 0, st>>>(a, p.pp, p.pt); break;
-    case 1: paged_prefix_kernel<DT, Slim<HD, 4>, MOD><<<n, 256, 0, st>>>(a, p.pp, p.pt); break;
-    case 2: paged_prefix_kernel<DT, Slim<HD, 2>, MOD><<<n, 128, 0, st>>>(a, p.pp, p.pt); break;
-    default: paged_prefix_kernel<DT, Slim<HD, 1>, MOD><<<n, 64, 0, st>>>(a, p.pp, p.pt); break;
-  }
-}
-template <int DT, int HD, bool MOD>
-void launch_seq(const Plan& p, const PagedAttn& a, hipStream_t st) {
-  const unsigned n = (unsigned)((int64_t)a.batch * a.nkv * p.nsplit * p.seq.blocks);
-#define PE_SEQ(C, W) \
-  paged_seq_kernel<DT, C, MOD><<<n, 64 * W, 0, st>>>(a, p.pp, p.pt, p.kps, p.nsplit, p.seq.blocks, 32u * p.seq.tiles)
-  switch (p.seq.kind) {
-    case 0: PE_SEQ(Wide<HD>, 8); break;
-    case 1: PE_SEQ(PE_ARG(Slim<HD, 4>), 4); break;
-    case 2: PE_SEQ(PE_ARG(Slim<HD, 2>), 2); break;
-    default: PE_SEQ(PE_ARG(Slim<HD, 1>), 1); break;
-  }
-#undef PE_SEQ
 }
 
 template <int DT, int HD, bool MOD>
 int launch_all(const Plan& p, const PagedAttn& a, hipStream_t st) {
-  if (a.prefix_len > 0) {
-    launch_prefix<DT, HD, MOD>(p, a, st);
+  if (p.wide) {
+    paged_prefix_kernel<DT, HD, MOD><<<(unsigned)p.pre_wgs, 512, 0, st>>>(a, p.pp, p.pt);
     PE_CHECK_LAUNCH();
   }
-  launch_seq<DT, HD, MOD>(p, a, st);
+  const uint32_t n_pre = p.wide ? 0 : (uint32_t)p.pre_wgs;
+  paged_attn_kernel<DT, HD, MOD><<<n_pre + (unsigned)p.items, 256, 0, st>>>(a, p.pp, p.pt, p.sq, n_pre, p.pre_kind);
   PE_CHECK_LAUNCH();
-  if (p.nsplit > 1) {
-    const int64_t rows = (int64_t)a.max_rows * (a.nh / a.nkv);
-    paged_join_kernel<DT, HD><<<dim3(pe_cdiv(rows, 1024 / HD), a.nkv, a.batch), 256, 0, st>>>(a, p.pp, p.pt, p.kps);
+  if (p.join) {
+    const int64_t tiles = ((int64_t)a.max_rows * (a.nh / a.nkv) + 31) / 32;
+    paged_join_kernel<DT, HD><<<dim3((unsigned)(tiles * (HD / 32)), a.nkv, a.batch), 256, 0, st>>>(a, p.pp, p.pt, p.sq);
     PE_CHECK_LAUNCH();
   }
   return PE_OK;
@@ -708,11 +741,11 @@ int64_t pe_internal_paged_mfma_bytes(int64_t M, int batch, int nh, int nkv, int 
 
 int pe_internal_paged_mfma(const PagedAttn& a, int dtype, void* workspace, int64_t workspace_bytes, hipStream_t st) {
   Plan p = make_plan(a.M, a.batch, a.nh, a.nkv, a.hd, a.max_rows, a.max_len, a.prefix_len);
-  if (workspace_bytes < p.o_bytes + p.ml_bytes || (p.parts > 0 && !workspace)) return PE_ERR_WORKSPACE;
+  if (p.o_bytes > 0 && (!workspace || workspace_bytes < p.o_bytes + p.ml_bytes)) return PE_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 15) return PE_ERR_ARG;
   // rows and work units are counted in 32 bits
   if (a.M * a.nh >= (int64_t(1) << 31) || p.units >= (int64_t(1) << 31) ||
-      (int64_t)a.batch * a.nkv * p.nsplit * p.seq.blocks >= (int64_t(1) << 31))
+      p.items >= (int64_t(1) << 30) || a.nkv > 65535)
     return PE_ERR_ARG;
   p.pt.o = (float*)workspace;
   p.pt.ml = (float*)((char*)workspace + p.o_bytes);
