@@ -25,6 +25,7 @@
 #include "pe_paged.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -60,24 +61,44 @@ __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
                                                    0, 0, 0);
 }
 
+// A row's two lanes (l and l ^ 32) joined: both get the larger value, or the sum.
+__device__ __forceinline__ float max_halves(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 // s_waitcnt with vmcnt = N, the other counters at their maxima
 template <int N>
 __device__ __forceinline__ void wait_vm() {
   __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
 }
 
-// One list of pages as the key source of a KV head.
-struct Pages {
+// The keys of an item: `pre_steps` steps of the prefix's `pre` keys (none: 0),
+// then the steps of a sequence's own keys [0, hi), P of them cached and new rows
+// after those. Keys are counted in 32 bits: a sequence is shorter than 2^30.
+struct Keys {
+  const int32_t* pre_table;
   const int32_t* table;
-  int lo, hi;  // keys read (counted in 32 bits: a sequence is shorter than 2^30), [lo, hi), the others of a step as the nearest
+  int pre_steps, pre;
+  int P, hi;
+  int base;      // position of key 0 of the sequence's own
+  int lo;        // first position that a row of the workgroup sees (0 without a window)
+  int new_rows;
+  int last;      // last own key that a row of the wave's tile sees
 };
 
 // What a lane's row needs besides its Q.
 struct RowInfo {
-  int node;       // causal: its token's index among the sequence's new rows; tree: unused
-  int rel;        // its position - the position of key 0 of the list (MOD)
-  float slope2;   // slope * log2 e (MOD)
-  int lo, tile_lo;  // first cached key its window holds; the largest of the tile's (MOD)
+  int node;         // causal: its token's index among the sequence's new rows
+  int pos;          // its position (MOD)
+  float slope2;     // slope * log2 e (MOD)
+  int lo, tile_lo;  // first position its window holds; the largest of the tile's (MOD)
   uint64_t nb0, nb1, nb2, nb3;  // ancestor bits (named: an indexed array would live in scratch memory)
 };
 static_assert(PE_TREE_MAX_WORDS == 4, "one field per word");
@@ -122,52 +143,54 @@ __device__ __forceinline__ uint64_t below(int n) {  // bits 0 .. n - 1
   return n >= 64 ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1);
 }
 
-// The keys [s0 SK, s1 SK) of a list for the workgroup's row tiles: O^T, m, l of
-// the wave's tile. `P`: the list's cached keys, new rows follow (PRE: no new rows).
-// Keys outside [pg.lo, pg.hi) are masked, steps past last_key (the last that a
-// row of the tile sees) skipped. npos (LDS): positions of the new rows relative
-// to key 0 (MOD, where distances count).
-template <int DT, typename C, bool MOD, bool PRE>
-__device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const Pages& pg, int kvh, int s0, int s1,
-                                       int P, int new_rows, bool live, int last_key, RowInfo ri,
-                                       const u32x4_t (&qf)[C::HD / 16], const int* npos, bool& bad,
-                                       f32x16_t (&o)[C::OB], float& m, float& l) {
+// The steps [s0, s1) of the keys for the workgroup's row tiles: O^T, m, l of the
+// wave's tile. Keys before k.lo and past a list's end are masked (their loads go
+// to the nearest key of the list that is read, so that no page outside it is
+// touched), steps past k.last skipped. npos (LDS): positions of the new rows of
+// a tree (MOD, where distances count).
+template <int DT, typename C, bool MOD>
+__device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const Keys& k, int kvh, int s0, int s1,
+                                       bool live, const RowInfo& ri, const u32x4_t (&qf)[C::HD / 16], const int* npos,
+                                       bool& bad, f32x16_t (&o)[C::OB], float& m, float& l) {
   constexpr int HD = C::HD, SB = C::SB, OB = C::OB;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int ln = lane & 31, g = lane >> 5, hb = (wave % C::DS) * OB;
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
   typedef const __attribute__((address_space(4))) int32_t* const_i32;  // read through the scalar cache
-  const const_i32 tab = (const_i32)(uintptr_t)uniform_ptr((const uint16_t*)pg.table);
+  const const_i32 tab_pre = (const_i32)(uintptr_t)uniform_ptr((const uint16_t*)k.pre_table);
+  const const_i32 tab_own = (const_i32)(uintptr_t)uniform_ptr((const uint16_t*)k.table);
   const int psl = a.ps_log2;
-  const int clo = pg.lo >> 4, chi = (pg.hi - 1) >> 4;
+  const int lo_pre = min(k.lo, max(k.pre - 1, 0)), lo_own = min(max(k.lo - k.base, 0), max(k.hi - 1, 0));
   // the pages of this wave's pieces of a step, asked for a step ahead
   int page[C::kChunks];
-  auto piece_of = [&](int step, int c) {
+  auto piece_of = [&](int step, int c) {  // its 16 keys' index in the step's list
+    const bool pre = step < k.pre_steps;
     const int ch = (wave * C::kChunks + c) % (C::SK / 16);
-    const int k = step * (C::SK / 16) + ch;
-    return k < clo ? clo : k > chi ? chi : k;
+    const int p = (pre ? step : step - k.pre_steps) * (C::SK / 16) + ch;
+    return max((pre ? lo_pre : lo_own) >> 4, min(p, ((pre ? k.pre : k.hi) - 1) >> 4));
   };
   auto ask = [&](int step) {
+    const const_i32 tab = step < k.pre_steps ? tab_pre : tab_own;
 #pragma unroll
     for (int c = 0; c < C::kChunks; ++c) page[c] = tab[(piece_of(step, c) << 4) >> psl];
   };
   auto issue = [&](int step) {
     const uint32_t buf = lds_base + (step % C::ST) * C::kStep;
+    const bool pre = step < k.pre_steps;
 #pragma unroll
     for (int c = 0; c < C::kChunks; ++c) {
       const int piece = wave * C::kChunks + c, ch = piece % (C::SK / 16);
       const bool is_v = piece >= C::SK / 16;
-      const int k16 = piece_of(step, c);
+      const int k16 = piece_of(step, c) << 4;
       int pgid = page[c];
       if (pgid < 0 || pgid >= a.num_pages) {
         bad = true;
         pgid = 0;
       }
-      const int64_t row = ((((int64_t)pgid * a.nkv + kvh) << psl) + ((k16 << 4) & ((1 << psl) - 1)));
+      const int64_t row = (((int64_t)pgid * a.nkv + kvh) << psl) + (k16 & ((1 << psl) - 1));
       const uint16_t* src = uniform_ptr((const uint16_t*)(is_v ? a.v_pool : a.k_pool) + row * HD);
-      const uint32_t dst =
-          __builtin_amdgcn_readfirstlane(buf + (is_v ? C::kHalf : 0) + ch * 16 * HD * 2);
-      const int rlo = max(pg.lo - (k16 << 4), 0), rhi = min(pg.hi - 1 - (k16 << 4), 15);
+      const uint32_t dst = __builtin_amdgcn_readfirstlane(buf + (is_v ? C::kHalf : 0) + ch * 16 * HD * 2);
+      const int rlo = max((pre ? lo_pre : lo_own) - k16, 0), rhi = min((pre ? k.pre : k.hi) - 1 - k16, 15);
 #pragma unroll
       for (int i = 0; i < C::kPerChunk; ++i) {
         constexpr int kLanes = HD / 8;  // lanes on a row
@@ -207,8 +230,9 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
       issue(s + C::ST - 1);
       if (s + C::ST < s1) ask(s + C::ST);
     }
-    const int kb0 = s * C::SK;
-    if (!live || kb0 > last_key) continue;  // wave-uniform: the tile sees no key of this step
+    const bool pre = s < k.pre_steps;
+    const int kb0 = (pre ? s : s - k.pre_steps) * C::SK, kpos = kb0 + (pre ? 0 : k.base);  // key 0 of the step
+    if (!live || (!pre && kb0 > k.last)) continue;  // wave-uniform: the tile sees no key of this step
     const uint8_t* kbp = smem + (s % C::ST) * C::kStep;
     const uint8_t* vbp = kbp + C::kHalf;
     f32x16_t sc[SB];
@@ -222,10 +246,10 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
       for (int sb = 0; sb < SB; ++sb)
         sc[sb] = mfma32<DT>(*(const u32x4_t*)(kbp + lds_at<HD>(32 * sb + ln, 2 * j + g)), qf[j], sc[sb]);
     // sc[sb][i] is key kb0 + 32 sb + 8 (i / 4) + 4 g + i % 4 of the lane's row
-    bool node_step = false;
-    if constexpr (!PRE) node_step = kb0 + 32 * SB > P;
+    const bool node_step = !pre && kb0 + 32 * SB > k.P;
     if constexpr (MOD) {
-      if (cap_in != 0.f) {
+      const bool capped = cap_in != 0.f, sloped = a.slopes != nullptr;
+      if (capped) {
         // cap tanh(s / cap) = cap (1 - 2 / (1 + e^(2 s / cap))): both ends exact
 #pragma unroll
         for (int sb = 0; sb < SB; ++sb)
@@ -234,41 +258,44 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
             const float e = __builtin_amdgcn_exp2f(sc[sb][i] * cap_in);
             sc[sb][i] = fmaf(-2.f * cap_out, __builtin_amdgcn_rcpf(1.f + e), cap_out);
           }
-      } else {
-#pragma unroll
-        for (int sb = 0; sb < SB; ++sb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sc[sb][i] *= scale2;
       }
-      const int d0 = ri.rel - kb0 - 4 * g;  // distance of key kb0 + 4 g
-      if (node_step && tree && npos) {  // new rows lie where their positions say
+      const int d0 = ri.pos - kpos - 4 * g;  // distance of key kb0 + 4 g
+      const float mul = capped ? 1.f : scale2;
+      if (node_step && npos) {  // a tree's new rows lie where their positions say
 #pragma unroll
         for (int sb = 0; sb < SB; ++sb)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int off = 32 * sb + 8 * (i >> 2) + (i & 3);
-            const int u = kb0 - P + off + 4 * g;
-            const int np = npos[max(0, min(u, new_rows - 1))];
-            const int dist = u < 0 ? d0 - off : ri.rel - np;
-            sc[sb][i] = fmaf(-ri.slope2, (float)dist, sc[sb][i]);
+            const int u = kb0 - k.P + off + 4 * g;
+            const int np = npos[max(0, min(u, k.new_rows - 1))];
+            const int dist = u < 0 ? d0 - off : ri.pos - np;
+            sc[sb][i] = fmaf(sc[sb][i], mul, -ri.slope2 * (float)dist);
             if (a.window > 0) sc[sb][i] = dist < a.window ? sc[sb][i] : -INFINITY;
           }
-      } else if (a.slopes) {
+      } else if (sloped) {
+        const float c0 = -ri.slope2 * (float)d0;
 #pragma unroll
         for (int sb = 0; sb < SB; ++sb)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            sc[sb][i] = fmaf(-ri.slope2, (float)(d0 - (32 * sb + 8 * (i >> 2) + (i & 3))), sc[sb][i]);
+            sc[sb][i] = fmaf(sc[sb][i], mul, fmaf(ri.slope2, (float)(32 * sb + 8 * (i >> 2) + (i & 3)), c0));
+      } else if (!capped) {
+#pragma unroll
+        for (int sb = 0; sb < SB; ++sb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[sb][i] *= scale2;
       }
     }
-    bool edge = node_step || kb0 + 32 * SB > pg.hi || kb0 < pg.lo;
-    if constexpr (MOD) edge = edge || kb0 < ri.tile_lo;
+    const int hi = pre ? k.pre : k.hi;
+    bool edge = node_step || kb0 + 32 * SB > hi;
+    if constexpr (MOD) edge = edge || kpos < ri.tile_lo;
     if (edge) {
       uint64_t win = ~0ull;
-      if constexpr (!PRE) win = tree ? node_window(kb0, P, ri.nb0, ri.nb1, ri.nb2, ri.nb3) : below(P + ri.node + 1 - kb0);
-      int lo = pg.lo;
-      if constexpr (MOD) lo = max(lo, ri.lo);
-      win &= below(pg.hi - kb0) & ~below(lo - kb0);
+      if (node_step)
+        win = tree ? node_window(kb0, k.P, ri.nb0, ri.nb1, ri.nb2, ri.nb3) : below(k.P + ri.node + 1 - kb0);
+      win &= below(hi - kb0);
+      if constexpr (MOD) win &= ~below(ri.lo - kpos);
       win >>= 4 * g;
 #pragma unroll
       for (int sb = 0; sb < SB; ++sb)
@@ -281,7 +308,7 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
     for (int sb = 0; sb < SB; ++sb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) bmax = fmaxf(bmax, sc[sb][i]);
-    bmax = fmaxf(bmax, __shfl_xor(bmax, 32, 64));
+    bmax = max_halves(bmax);
     if constexpr (!MOD) bmax *= scale2;
     const float mnew = fmaxf(m, bmax);
     const float alpha = __builtin_amdgcn_exp2f(m - mnew);
@@ -296,8 +323,7 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
         psum += p0 + p1;
         pb[sb][i >> 1] = pack2_16<DT>(p0, p1);
       }
-    psum += __shfl_xor(psum, 32, 64);
-    l = l * alpha + psum;
+    l = l * alpha + psum;  // of the lane's half of the keys: the halves are joined at the end
     if (__builtin_amdgcn_ballot_w64(mnew != m) != 0ull) {
 #pragma unroll
       for (int h = 0; h < OB; ++h)
@@ -327,6 +353,292 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
       }
     }
   }
+  l = sum_halves(l);
+}
+
+// ---------------------------------------------------------------------------
+// The prefix's wide blocks: eight waves, two to a SIMD, in opposite phases
+// ---------------------------------------------------------------------------
+// A step of a wave is 32 matrix instructions (1024 cycles of the matrix core)
+// and about as many cycles of exponentials and other vector work. In step with
+// each other, the two waves of a SIMD would compete for the one and then for the
+// other: the same kernel with one barrier a step ran at 37% of the matrix
+// core's rate. So waves 0 - 3 and 4 - 7 work in turns. Phase X of a step: O^T +=
+// V^T P^T of the step before, then S^T = K Q^T; phase Y: softmax of S, O's
+// rescaling. A barrier ends each phase; group 0 is in X when group 1 is in Y.
+//
+// In phases counted from the start of the item, group e does X of step i in
+// phase 2 i + e and Y in the next; V of step i is last read in phase 2 i + 3. In
+// every even phase 2 i all waves request step i + 2 into the ring's buffer of
+// step i - 2 (free since the barrier that ended phase 2 i - 1) and wait for
+// step i + 1's at the end of the next phase, so two steps are in flight.
+//
+// LDS reads run two groups of four matrix instructions ahead of their use.
+// A row's running maximum follows its block's only when it is passed by more
+// than 2^8 (kSlack): O and l are sums of the same 2^(s - m), whichever m, and the
+// weights, at most 2^8, lose nothing in fp32 nor when rounded (fp16's largest
+// value is 2^16); O's 64 products a step are mostly saved.
+constexpr float kSlack = 8.f;
+
+template <int DT, typename C, bool MOD>
+__device__ __forceinline__ void attend_wide(const PagedAttn& a, uint8_t* smem, const int32_t* table, int n, int lo,
+                                            int kvh, int s0, int s1, bool live, const RowInfo& ri,
+                                            const u32x4_t (&qf)[C::HD / 16], bool& bad, f32x16_t (&o)[C::HD / 32],
+                                            float& m, float& l) {
+  constexpr int HD = C::HD, NJ = HD / 16, NH = HD / 32;
+  static_assert(C::W == 8 && C::SB == 2 && C::ST == 4 && C::kChunks == 1, "the schedule above");
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int ln = lane & 31, g = lane >> 5, grp = wave >> 2;
+  const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+  typedef const __attribute__((address_space(4))) int32_t* const_i32;
+  const const_i32 tab = (const_i32)(uintptr_t)uniform_ptr((const uint16_t*)table);
+  const int psl = a.ps_log2, lo_k = min(lo, n - 1);
+  const int ch = wave & 3;  // this wave's 16 keys of K (waves 0 - 3) or V of a step
+  const uint16_t* pool = (const uint16_t*)(grp ? a.v_pool : a.k_pool);
+  int page = 0;
+  auto piece_of = [&](int step) { return max(lo_k >> 4, min(step * 4 + ch, (n - 1) >> 4)); };
+  auto ask = [&](int step) { page = tab[(piece_of(step) << 4) >> psl]; };
+  auto issue = [&](int step) {
+    const int k16 = piece_of(step) << 4;
+    int pgid = page;
+    if (pgid < 0 || pgid >= a.num_pages) {
+      bad = true;
+      pgid = 0;
+    }
+    const int64_t row = (((int64_t)pgid * a.nkv + kvh) << psl) + (k16 & ((1 << psl) - 1));
+    const uint16_t* src = uniform_ptr(pool + row * HD);
+    const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_base + (step & 3) * C::kStep + grp * C::kHalf + ch * 16 * HD * 2);
+    const int rlo = max(lo_k - k16, 0), rhi = min(n - 1 - k16, 15);
+#pragma unroll
+    for (int i = 0; i < C::kPerChunk; ++i) {
+      constexpr int kLanes = HD / 8;
+      const int r = i * (64 / kLanes) + lane / kLanes;
+      lds_dma16(src, (uint32_t)(min(max(r, rlo), rhi) * (HD * 2) + (((lane % kLanes) ^ swizzle<HD>(r)) << 4)), dst + i * 1024);
+    }
+  };
+
+#pragma unroll
+  for (int h = 0; h < NH; ++h)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[h][i] = 0.f;
+  m = kPagedInitMax;
+  l = 0.f;
+  const float scale2 = a.scale * kLog2e;
+  const float cap_in = MOD && a.softcap > 0.f ? 2.f * scale2 / a.softcap : 0.f, cap_out = a.softcap * kLog2e;
+  f32x16_t sc[2];
+  uint32_t pb[2][8];
+#pragma unroll
+  for (int sb = 0; sb < 2; ++sb) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) pb[sb][i] = 0u;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sc[sb][i] = 0.f;
+  }
+  // the lane's LDS offsets: K row ln of a 32-key half, and V's transposed reads
+  const int qg = lane >> 4, jl = lane & 15, vrow = 4 * (qg >> 1) + (jl >> 2), vcol = 16 * (qg & 1) + 4 * (jl & 3);
+  uint32_t k_at[NJ], v_at[2][NH];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) k_at[j] = lds_at<HD>(ln, 2 * j + g);
+#pragma unroll
+  for (int h = 0; h < NH; ++h) {
+    v_at[0][h] = lds_at<HD>(vrow, (32 * h + vcol) >> 3) + (vcol & 7) * 2;
+    v_at[1][h] = lds_at<HD>(vrow + 8, (32 * h + vcol) >> 3) + (vcol & 7) * 2;
+  }
+  typedef short s4v_t __attribute__((__vector_size__(4 * sizeof(short))));
+  typedef __attribute__((address_space(3))) s4v_t lds_s4v_t;
+
+  // Phase X: `pv`: step s - 1's P V, `qk`: step s's scores. Groups of LDS reads
+  // 0 .. 3: V of a 16-key quarter (4 products of hd 128, 2 of 64), then K, as
+  // many products a group.
+  auto phase_x = [&](int s, bool pv, bool qk) {
+    const uint8_t* vbp = smem + ((s - 1) & 3) * C::kStep + C::kHalf;
+    const uint8_t* kbp = smem + (s & 3) * C::kStep;
+    constexpr int kG = 4 + 4;  // groups
+    u32x4_t f[3][NH];
+    auto read = [&](int gr) {
+      if (gr < 4) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                        (lds_s4v_t*)(vbp + v_at[0][h] + gr * 16 * HD * 2)));
+          const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                        (lds_s4v_t*)(vbp + v_at[1][h] + gr * 16 * HD * 2)));
+          f[gr % 3][h] = u32x4_t{x.x, x.y, y.x, y.y};
+        }
+      } else if (gr < kG) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          const int at = (gr - 4) * NH + h;  // product 2 j + sb
+          f[gr % 3][h] = *(const u32x4_t*)(kbp + k_at[at >> 1] + (at & 1) * 32 * HD * 2);
+        }
+      }
+    };
+    auto mul = [&](int gr) {
+      if (gr < 4) {
+        const int sb = gr >> 1, q = gr & 1;
+        const u32x4_t bp = {pb[sb][4 * q], pb[sb][4 * q + 1], pb[sb][4 * q + 2], pb[sb][4 * q + 3]};
+#pragma unroll
+        for (int h = 0; h < NH; ++h) o[h] = mfma32<DT>(f[gr % 3][h], bp, o[h]);
+      } else {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          const int at = (gr - 4) * NH + h;
+          if (at < 2)
+            sc[at] = mfma32<DT>(f[gr % 3][h], qf[0], f32x16_t{});
+          else
+            sc[at & 1] = mfma32<DT>(f[gr % 3][h], qf[at >> 1], sc[at & 1]);
+        }
+      }
+    };
+    static_assert(4 * NH == 2 * NJ, "four groups of K");
+    const int g0 = pv ? 0 : 4, g1 = qk ? kG : 4;
+    // three bodies, so that each is straight code
+    auto run = [&](auto from, auto to) {
+      constexpr int F = decltype(from)::value, T = decltype(to)::value;
+      read(F);
+      if constexpr (F + 1 < T) read(F + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int gr = F; gr < T; ++gr) {
+        if (gr + 2 < T) read(gr + 2);
+        __builtin_amdgcn_sched_barrier(0);
+        mul(gr);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    if (g0 == 0 && g1 == kG) run(std::integral_constant<int, 0>{}, std::integral_constant<int, kG>{});
+    else if (g0 == 0) run(std::integral_constant<int, 0>{}, std::integral_constant<int, 4>{});
+    else run(std::integral_constant<int, 4>{}, std::integral_constant<int, kG>{});
+  };
+
+  auto phase_y = [&](int s) {
+    const int kb0 = s * 64;
+    if constexpr (MOD) {
+      const bool capped = cap_in != 0.f;
+      if (capped) {
+#pragma unroll
+        for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float e = __builtin_amdgcn_exp2f(sc[sb][i] * cap_in);
+            sc[sb][i] = fmaf(-2.f * cap_out, __builtin_amdgcn_rcpf(1.f + e), cap_out);
+          }
+      }
+      const float mul = capped ? 1.f : scale2;
+      if (a.slopes) {
+        const float c0 = -ri.slope2 * (float)(ri.pos - kb0 - 4 * g);
+#pragma unroll
+        for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            sc[sb][i] = fmaf(sc[sb][i], mul, fmaf(ri.slope2, (float)(32 * sb + 8 * (i >> 2) + (i & 3)), c0));
+      } else if (!capped) {
+#pragma unroll
+        for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[sb][i] *= scale2;
+      }
+    }
+    bool edge = kb0 + 64 > n;
+    if constexpr (MOD) edge = edge || kb0 < ri.tile_lo;
+    if (edge) {
+      uint64_t win = below(n - kb0);
+      if constexpr (MOD) win &= ~below(ri.lo - kb0);
+      win >>= 4 * g;
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          sc[sb][i] = ((win >> (32 * sb + 8 * (i >> 2) + (i & 3))) & 1ull) ? sc[sb][i] : -INFINITY;
+    }
+    float bmax = -INFINITY;
+#pragma unroll
+    for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) bmax = fmaxf(bmax, sc[sb][i]);
+    bmax = max_halves(bmax);
+    if constexpr (!MOD) bmax *= scale2;
+    if (__builtin_amdgcn_ballot_w64(bmax > m + kSlack) != 0ull) {
+      const float mnew = fmaxf(m, bmax);
+      const float alpha = __builtin_amdgcn_exp2f(m - mnew);
+      l *= alpha;
+      m = mnew;
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[h][i] *= alpha;
+    }
+    float psum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(MOD ? sc[sb][i] - m : fmaf(sc[sb][i], scale2, -m));
+        const float p1 = __builtin_amdgcn_exp2f(MOD ? sc[sb][i + 1] - m : fmaf(sc[sb][i + 1], scale2, -m));
+        psum[0] += p0;
+        psum[1] += p1;
+        pb[sb][i >> 1] = pack2_16<DT>(p0, p1);
+      }
+    l += psum[0] + psum[1];  // of the lane's half of the keys: the halves are joined at the end
+  };
+
+  // a phase's start and end: requests in even phases, waits at the end of odd ones
+  const int steps = s1 - s0;
+  auto enter = [&](int phase) {
+    if (!(phase & 1)) {
+      const int st = s0 + (phase >> 1) + 2;
+      if (st < s1) {
+        issue(st);
+        if (st + 1 < s1) ask(st + 1);
+      }
+    }
+  };
+  auto leave = [&](int phase) {
+    if (phase & 1) {
+      // step (phase + 1) / 2 is read from the next phase on; the one after it may still be in flight
+      if (s0 + (phase >> 1) + 2 < s1) wait_vm<C::kLoads>();
+      else wait_vm<0>();
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  if (steps <= 0) return;
+  ask(s0);
+  __syncthreads();  // the buffers' last readers are done
+  issue(s0);
+  if (s0 + 1 < s1) {
+    ask(s0 + 1);
+    issue(s0 + 1);
+    if (s0 + 2 < s1) ask(s0 + 2);
+  }
+  __builtin_amdgcn_s_waitcnt(0);  // Q has landed: no later wait of the compiler's covers the ring's loads
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  int phase = 0;
+  if (grp) {
+    enter(phase);
+    leave(phase);
+    ++phase;
+  }
+  for (int i = 0; i < steps; ++i) {
+    enter(phase);
+    if (live) {
+      __builtin_amdgcn_s_setprio(1);
+      phase_x(s0 + i, i > 0, true);
+      __builtin_amdgcn_s_setprio(0);
+    }
+    leave(phase);
+    ++phase;
+    enter(phase);
+    if (live) phase_y(s0 + i);
+    leave(phase);
+    ++phase;
+  }
+  if (live) phase_x(s1, true, false);
+  if (!grp) leave(phase + 1);  // the other group's last phases
+  l = sum_halves(l);
 }
 
 // Work item of workgroup `b` of `n`: neighbours in the sequence of items (which
@@ -356,27 +668,25 @@ __device__ __forceinline__ void store_part(const PagedParts& p, int nkv, int par
   }
 }
 
-// The lane's row's first cached key inside its window (ri.lo), the last of the
-// tile's (ri.tile_lo) and the first of the workgroup's (returned); `cached` keys.
+// The first position that the lane's row sees (ri.lo, at most `end`), the last
+// of the tile's (ri.tile_lo) and the first of the workgroup's (returned).
 template <int W>
-__device__ __forceinline__ int window_lo(const PagedAttn& a, RowInfo& ri, int cached, bool live, int* s_lo) {
+__device__ __forceinline__ int window_lo(const PagedAttn& a, RowInfo& ri, int end, bool live, int* s_lo) {
   ri.lo = ri.tile_lo = 0;
   if (a.window == 0) return 0;
-  ri.lo = (int)min(max((int64_t)ri.rel - a.window + 1, (int64_t)0), (int64_t)cached);
-  int lo = live ? ri.lo : cached, hi = ri.lo;
+  ri.lo = (int)min(max((int64_t)ri.pos - a.window + 1, (int64_t)0), (int64_t)end);
+  int lo = live ? ri.lo : end, hi = ri.lo;
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) {
     lo = min(lo, __shfl_xor(lo, d, 64));
     hi = max(hi, __shfl_xor(hi, d, 64));
   }
   ri.tile_lo = __builtin_amdgcn_readfirstlane(hi);
-  if constexpr (W > 1) {
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) s_lo[threadIdx.x >> 6] = lo;
-    __syncthreads();
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s_lo[threadIdx.x >> 6] = lo;
+  __syncthreads();
 #pragma unroll
-    for (int i = 0; i < W; ++i) lo = min(lo, s_lo[i]);
-  }
+  for (int i = 0; i < W; ++i) lo = min(lo, s_lo[i]);
   return __builtin_amdgcn_readfirstlane(lo);
 }
 
@@ -395,8 +705,9 @@ __device__ __forceinline__ void prefix_share(const PagedAttn& a, const PagedPref
   for (uint32_t u = w * pp.per; u < uend;) {
     const uint32_t x = u / pp.steps;
     const int s0 = (int)(u - x * pp.steps);
-    const int s1 = (int)min(pp.steps, s0 + (uend - u));
-    u += s1 - s0;
+    const uint32_t past = min(pp.steps, s0 + (uend - u));  // a block's last steps may be beyond its keys
+    u += past - s0;
+    const int s1 = min((int)past, ((int)a.prefix_len - 1) / C::SK + 1);
     const int kvh = (int)(x / pp.nblk);
     const uint32_t blk0 = (x - kvh * pp.nblk) * pp.block_rows, row0 = blk0 + 32 * tile;
     const bool live = row0 < min(blk0 + pp.block_rows, R);
@@ -408,18 +719,20 @@ __device__ __forceinline__ void prefix_share(const PagedAttn& a, const PagedPref
     for (int j = 0; j < HD / 16; ++j) qf[j] = *(const u32x4_t*)(qr + 16 * j);
     RowInfo ri;
     const int S0 = (int)a.prefix_len;
-    Pages pg{a.prefix_table, 0, S0};
+    Keys k{a.prefix_table, a.prefix_table, 1 << 30, S0, 0, 0, S0, 0, 0, 0};
     int first = s0;
     if constexpr (MOD) {
-      ri.rel = a.positions ? (int)a.positions[tok] : 0;
+      ri.pos = a.positions ? (int)a.positions[tok] : 0;
       ri.slope2 = a.slopes ? a.slopes[hq] * kLog2e : 0.f;
-      const int lo = window_lo<C::W>(a, ri, S0, live, s_lo);
-      pg.lo = min(lo, S0 - 1);
-      if (lo > 0) first = lo >= S0 ? s1 : max(s0, lo / C::SK);  // steps behind every row's window
+      k.lo = window_lo<C::W>(a, ri, S0, live, s_lo);
+      if (k.lo > 0) first = k.lo >= S0 ? s1 : max(s0, k.lo / C::SK);  // steps behind every row's window
     }
     f32x16_t o[C::OB];
     float m, l;
-    attend<DT, C, MOD, true>(a, smem, pg, kvh, first, max(first, s1), S0, 0, live, S0 - 1, ri, qf, nullptr, bad, o, m, l);
+    if constexpr (C::W == 8)
+      attend_wide<DT, C, MOD>(a, smem, a.prefix_table, S0, k.lo, kvh, first, s1, live, ri, qf, bad, o, m, l);
+    else
+      attend<DT, C, MOD>(a, smem, k, kvh, first, max(first, s1), live, ri, qf, nullptr, bad, o, m, l);
     if (live)
       store_part<HD, C::OB>(parts, a.nkv, (int)(w - prefix_first_wg(pp, x)), kvh, row0 + ln, g, hb, o, m, l);
   }
@@ -427,17 +740,23 @@ __device__ __forceinline__ void prefix_share(const PagedAttn& a, const PagedPref
 }
 
 // ---------------------------------------------------------------------------
-// The sequences' own keys: item = (key split of kps keys, sequence, KV head,
-// block of row tiles)
+// The sequences' own keys: item = (key split, sequence, KV head, block of row
+// tiles)
 // ---------------------------------------------------------------------------
-// The launch's shares of it. `direct`: a sequence of one split joins the
+// The launch's shares of it, in key steps of `step` keys: the prefix's
+// `pre_steps` first where the items take it themselves (a prefix that is short
+// beside a sequence's rows: its parts would cost more than reading it again),
+// then the sequence's own. `direct`: a sequence of one split joins the
 // prefix's parts of its rows to its own (an earlier launch wrote them, and they
 // are few) and writes the output; otherwise its result is a part as well and
 // paged_join_kernel writes the output.
 struct PagedSeqs {
-  uint32_t items, kps, nblk, block_rows;
-  int nsplit, kind, direct;
+  uint32_t items, nblk, block_rows;
+  int split_steps, pre_steps, step, nsplit, kind, direct;
 };
+__device__ __forceinline__ int splits_of(const PagedSeqs& sq, const PagedSeq& s) {
+  return (sq.pre_steps + ((int)s.priv + s.rows - 1) / sq.step) / sq.split_steps + 1;
+}
 
 template <int DT, int OB>
 __device__ __forceinline__ void write_out(const PagedAttn& a, int64_t tok, int64_t col, const f32x16_t (&o)[OB],
@@ -480,7 +799,7 @@ __device__ __forceinline__ void seq_item(const PagedAttn& a, const PagedPrefix& 
   const uint32_t G = (uint32_t)(a.nh / a.nkv), R = T * G;
   const int P = (int)s.priv, S = P + T;
   const uint32_t blk0 = blk * sq.block_rows;
-  const int my_splits = (int)(((uint32_t)S + sq.kps - 1) / sq.kps);
+  const int my_splits = splits_of(sq, s);
   if (blk0 >= R || split >= my_splits) return;
   const int ln = lane & 31, g = lane >> 5, tile = wave / C::DS, hb = (wave % C::DS) * C::OB;
   const bool tree = a.mask_mode == PE_MASK_TREE;
@@ -507,22 +826,26 @@ __device__ __forceinline__ void seq_item(const PagedAttn& a, const PagedPrefix& 
   // the keys some row of the block sees end at hi; of this wave's tile, at last_key
   const int t_blk = min(T - 1, (int)((blk0 + sq.block_rows - 1) / G));
   const int t_tile = min(T - 1, (int)((row0 + 31) / G));
-  Pages pg{a.block_table + b * a.ld_table, 0, tree ? S : P + t_blk + 1};
-  const int last_key = tree ? S - 1 : P + t_tile;
+  const int S0 = (int)a.prefix_len;
+  Keys k{a.prefix_table, a.block_table + b * a.ld_table, sq.pre_steps, sq.pre_steps ? S0 : 0, P,
+         tree ? S : P + t_blk + 1, S0, 0, T, tree ? S - 1 : P + t_tile};
+  const int s_end = sq.pre_steps + (k.hi + C::SK - 1) / C::SK;
+  int s0 = split * sq.split_steps;
+  const int s1 = min(s_end, s0 + sq.split_steps);
   if constexpr (MOD) {
-    ri.rel = a.positions ? (int)(a.positions[tok] - a.prefix_len) : 0;
+    ri.pos = a.positions ? (int)a.positions[tok] : 0;
     ri.slope2 = a.slopes ? a.slopes[hq] * kLog2e : 0.f;
     if (a.positions && tree)
-      for (int u = tid; u < T; u += 64 * C::W) s_npos[u] = (int)(a.positions[s.row0 + u] - a.prefix_len);
-    pg.lo = window_lo<C::W>(a, ri, tree ? P : pg.hi - 1, live, s_lo);
+      for (int u = tid; u < T; u += 64 * C::W) s_npos[u] = (int)a.positions[s.row0 + u];
+    k.lo = window_lo<C::W>(a, ri, S0 + (tree ? P : k.hi - 1), live, s_lo);
+    if (k.lo >= S0) s0 = max(s0, sq.pre_steps + (k.lo - S0) / C::SK);  // steps behind every row's window
+    else if (sq.pre_steps) s0 = max(s0, k.lo / C::SK);
   }
-  const int k0 = split * (int)sq.kps, k1 = min(pg.hi, k0 + (int)sq.kps);
-  const int s1 = (k1 + C::SK - 1) / C::SK, s0 = max(k0, pg.lo) / C::SK;
   bool bad = false;
   f32x16_t o[C::OB];
   float m, l;
-  attend<DT, C, MOD, false>(a, smem, pg, kvh, s0, max(s0, s1), P, T, live, last_key, ri, qf,
-                            MOD && a.positions ? s_npos : nullptr, bad, o, m, l);
+  attend<DT, C, MOD>(a, smem, k, kvh, s0, max(s0, s1), live, ri, qf, MOD && a.positions && tree ? s_npos : nullptr, bad, o,
+                     m, l);
   if (bad && lane == 0) atomicOr(a.status, PE_ERR_INDEX);
   if (row0 + ln >= row_end) return;
   const uint32_t grow = (uint32_t)s.row0 * G + row;  // the row among the whole batch's
@@ -602,7 +925,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefi
   const int b = blockIdx.z, kvh = blockIdx.y;
   const PagedSeq s = paged_seq(a, b);
   if (!s.ok) return;
-  const int my_splits = (int)(((uint32_t)(s.priv + s.rows) + sq.kps - 1) / sq.kps);
+  const int my_splits = splits_of(sq, s);
   const uint32_t G = (uint32_t)(a.nh / a.nkv), R = s.rows * G;
   const uint32_t row = blockIdx.x / (HD / 32) * 32 + (threadIdx.x & 31);
   const int piece = (int)(blockIdx.x % (HD / 32)) * 8 + (int)(threadIdx.x >> 5);  // dims 4 piece .. + 3
@@ -614,7 +937,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefi
   const float2* sml = (const float2*)parts.ml + (int64_t)kvh * parts.tiles * 32 + grow;
   const int64_t o_part = (int64_t)a.nkv * parts.tiles * (32 * HD), ml_part = (int64_t)a.nkv * parts.tiles * 32;
   float m = kPagedInitMax, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  constexpr int kAhead = 4;  // parts asked for before the first is joined
+  constexpr int kAhead = 8;  // parts asked for before the first is joined
   const int n = npre + my_splits;
   for (int i0 = 0; i0 < n; i0 += kAhead) {
     float2 ml[kAhead];
@@ -646,7 +969,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefi
 
 // ------------------------------------------------------------------ plans
 constexpr int kCus = 256;
-constexpr int kSeqWgs = 2048, kMinSplit = 256, kSplitRows = 8, kPrefixSteps = 4, kFusedPre = 256;
+constexpr int kSeqWgs = 1024, kMinSplit = 64, kSplitRows = 2, kPrefixSteps = 4, kFusedPre = 256, kFoldKeys = 64;
 constexpr int64_t kWideUnits = 4096;
 
 // A launch's workgroups: which configuration, row tiles per block and how many
@@ -681,32 +1004,41 @@ Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int6
   p.pre_wgs = p.units = 0;
   p.pt.pre_parts = p.pre_kind = 0;
   p.wide = false;
-  if (prefix_len > 0) {
+  const Shape seq = shape_of(((int64_t)max_rows * G + 31) / 32, 4);
+  const int step = step_keys(seq, hd);
+  const bool fold = prefix_len <= std::max<int64_t>(kFoldKeys, max_rows * G);
+  const int64_t pre_steps = fold ? (prefix_len + step - 1) / step : 0;
+  if (!fold) {
     const int64_t s64 = (prefix_len - 1) / 64 + 1;
     // many rows over many keys: the wide blocks' own launch
     p.wide = tiles > 4 && tiles * s64 * nkv >= kWideUnits * 8;
     const Shape pre = shape_of(tiles, p.wide ? 8 : 4);
     p.pre_kind = pre.kind;
     const int64_t steps = (prefix_len - 1) / step_keys(pre, hd) + 1, blocks = nkv * pre.blocks;
-    p.units = blocks * steps;
-    const int64_t want = std::min<int64_t>(p.wide ? kCus : kFusedPre, std::max(blocks, p.units / kPrefixSteps));
-    const int64_t per = (p.units + want - 1) / want;
-    p.pp = PagedPrefix{(uint32_t)p.units, (uint32_t)per, (uint32_t)steps, (uint32_t)pre.blocks, (uint32_t)(32 * pre.tiles)};
-    p.pre_wgs = (p.units + per - 1) / per;
-    p.pt.pre_parts = (int)((steps - 1) / per) + 2;
+    if (p.wide) {
+      p.units = blocks * steps;
+      const int64_t per = (p.units + kCus - 1) / kCus;
+      p.pp = PagedPrefix{(uint32_t)p.units, (uint32_t)per, (uint32_t)steps, (uint32_t)pre.blocks, (uint32_t)(32 * pre.tiles)};
+      p.pt.pre_parts = (int)((steps - 1) / per) + 2;
+    } else {
+      const int64_t k = std::max<int64_t>(1, std::min<int64_t>(kFusedPre / blocks, steps / kPrefixSteps));
+      const int64_t per = (steps + k - 1) / k, parts = (steps + per - 1) / per;
+      p.units = blocks * per * parts;
+      p.pp = PagedPrefix{(uint32_t)p.units, (uint32_t)per, (uint32_t)(per * parts), (uint32_t)pre.blocks,
+                         (uint32_t)(32 * pre.tiles)};
+      p.pt.pre_parts = (int)parts;
+    }
+    p.pre_wgs = (p.units + p.pp.per - 1) / p.pp.per;
   }
-  const Shape seq = shape_of(((int64_t)max_rows * G + 31) / 32, 4);
-  const int64_t keys = max_len - prefix_len + max_rows;
+  const int64_t steps = pre_steps + (max_len - prefix_len + max_rows - 1) / step + 1;
   const int64_t wgs = batch * nkv * seq.blocks;
   const int64_t least = std::max<int64_t>(kMinSplit, kSplitRows * std::min<int64_t>(32 * seq.tiles, max_rows * G));
-  int64_t ns = std::max(std::min<int64_t>(2 * kCus / wgs, keys / kMinSplit), std::min<int64_t>(kSeqWgs / wgs, keys / least));
-  ns = std::max<int64_t>(1, ns);
-  const int64_t kps = (((keys + ns - 1) / ns + 63) / 64) * 64;
-  const int64_t nsplit = (keys + kps - 1) / kps;
+  const int64_t ns = std::max<int64_t>(1, std::min<int64_t>(kSeqWgs / wgs, steps * step / least));
+  const int64_t split_steps = (steps + ns - 1) / ns, nsplit = (steps + split_steps - 1) / split_steps;
   p.items = wgs * nsplit;
-  const bool direct = prefix_len == 0 || (p.wide && p.pt.pre_parts <= 3);
-  p.sq = PagedSeqs{(uint32_t)p.items, (uint32_t)kps, (uint32_t)seq.blocks, (uint32_t)(32 * seq.tiles), (int)nsplit, seq.kind,
-                   direct};
+  const bool direct = fold || (p.wide && p.pt.pre_parts <= 3);
+  p.sq = PagedSeqs{(uint32_t)p.items, (uint32_t)seq.blocks, (uint32_t)(32 * seq.tiles), (int)split_steps, (int)pre_steps,
+                   step, (int)nsplit, seq.kind, direct};
   p.join = nsplit > 1 || !direct;
   const int64_t parts = p.pt.pre_parts + (p.join ? nsplit : 0);
   p.o_bytes = parts * nkv * tiles * 32 * hd * 4;

@@ -72,10 +72,10 @@ class Case:
         self.ks, self.vs = [], []
 
         def put(tab, ktok, vtok):
-            for j in range(ktok.shape[0]):
-                p = int(tab[j // page])
-                k[p, :, j % page] = ktok[j]
-                v[p, :, j % page] = vtok[j]
+            j = torch.arange(ktok.shape[0])
+            at = tab[j // page].long()
+            k[at, :, j % page] = ktok
+            v[at, :, j % page] = vtok
 
         put(ptab, self.kpre, self.vpre)
         for b in range(B):
@@ -232,6 +232,16 @@ def test_long_keys_of_few_rows(heads, dtype):
 def test_many_rows_of_one_prefix(heads, dtype):
     """Row blocks of the prefix that end inside a sequence and inside a tile."""
     c = Case(heads, [26] * 11 + [31], [i for i in range(12)], 333, dtype=dtype, seed=6)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("cap,window,bias", [(0.0, 0, False), (40.0, 0, True), (0.0, 1500, False)])
+@pytest.mark.parametrize("heads,dtype,seqs,prefix", [((40, 8, 128), torch.bfloat16, 16, 4133), ((16, 16, 64), torch.float16, 33, 5121)],
+                         ids=["14b", "64"])
+def test_many_rows_over_a_long_prefix(heads, dtype, seqs, prefix, cap, window, bias):
+    """The prefix's own launch (row blocks of 256, two groups of waves in opposite phases)."""
+    c = Case(heads, [26] * (seqs - 1) + [9], [(37 * i) % 300 for i in range(seqs)], prefix, page=64, dtype=dtype, seed=10,
+             cap=cap, window=window, bias=bias)
     c.check(c.run())
 
 
