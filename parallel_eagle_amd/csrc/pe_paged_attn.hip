@@ -368,10 +368,12 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
 // rescaling. A barrier ends each phase; group 0 is in X when group 1 is in Y.
 //
 // In phases counted from the start of the item, group e does X of step i in
-// phase 2 i + e and Y in the next; V of step i is last read in phase 2 i + 3. In
-// every even phase 2 i all waves request step i + 2 into the ring's buffer of
-// step i - 2 (free since the barrier that ended phase 2 i - 1) and wait for
-// step i + 1's at the end of the next phase, so two steps are in flight.
+// phase 2 i + e and Y in the next. Group 0 loads the steps' K, group 1 their V,
+// each in its phases Y (X is the longer one): in Y of step i what step i + 2
+// needs, into the ring's buffer of step i - 2. K(i - 2) was last read in phase
+// 2 i - 3 and V(i - 2) in 2 i - 1, both before those phases (2 i + 1 and 2 i + 2).
+// K(i + 1) has to be there at the end of phase 2 i + 1 and V(i) as well: the
+// loads issued after those are one step's, so two steps are in flight.
 //
 // LDS reads run two groups of four matrix instructions ahead of their use.
 // A row's running maximum follows its block's only when it is passed by more
@@ -582,21 +584,11 @@ __device__ __forceinline__ void attend_wide(const PagedAttn& a, uint8_t* smem, c
     l += psum[0] + psum[1];  // of the lane's half of the keys: the halves are joined at the end
   };
 
-  // a phase's start and end: requests in even phases, waits at the end of odd ones
+  // the end of a phase; `landed`: this wave's loads but the last step's have to be there
   const int steps = s1 - s0;
-  auto enter = [&](int phase) {
-    if (!(phase & 1)) {
-      const int st = s0 + (phase >> 1) + 2;
-      if (st < s1) {
-        issue(st);
-        if (st + 1 < s1) ask(st + 1);
-      }
-    }
-  };
-  auto leave = [&](int phase) {
-    if (phase & 1) {
-      // step (phase + 1) / 2 is read from the next phase on; the one after it may still be in flight
-      if (s0 + (phase >> 1) + 2 < s1) wait_vm<C::kLoads>();
+  auto leave = [&](bool landed, bool later) {
+    if (landed) {
+      if (later) wait_vm<C::kLoads>();
       else wait_vm<0>();
     }
     asm volatile("" ::: "memory");
@@ -613,31 +605,25 @@ __device__ __forceinline__ void attend_wide(const PagedAttn& a, uint8_t* smem, c
     if (s0 + 2 < s1) ask(s0 + 2);
   }
   __builtin_amdgcn_s_waitcnt(0);  // Q has landed: no later wait of the compiler's covers the ring's loads
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-  int phase = 0;
-  if (grp) {
-    enter(phase);
-    leave(phase);
-    ++phase;
-  }
+  leave(false, false);
+  if (grp) leave(false, false);
   for (int i = 0; i < steps; ++i) {
-    enter(phase);
     if (live) {
       __builtin_amdgcn_s_setprio(1);
       phase_x(s0 + i, i > 0, true);
       __builtin_amdgcn_s_setprio(0);
     }
-    leave(phase);
-    ++phase;
-    enter(phase);
+    leave(grp, i + 1 < steps);  // group 1: V of step i
+    const int st = s0 + i + 2;
+    if (st < s1) {
+      issue(st);
+      if (st + 1 < s1) ask(st + 1);
+    }
     if (live) phase_y(s0 + i);
-    leave(phase);
-    ++phase;
+    leave(!grp, st < s1);  // group 0: K of step i + 1
   }
   if (live) phase_x(s1, true, false);
-  if (!grp) leave(phase + 1);  // the other group's last phases
+  if (!grp) leave(false, false);  // the other group's last phase but one
   l = sum_halves(l);
 }
 
