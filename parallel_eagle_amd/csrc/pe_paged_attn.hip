@@ -79,6 +79,51 @@ __device__ __forceinline__ void wait_vm() {
   __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
 }
 
+typedef short s4v_t __attribute__((__vector_size__(4 * sizeof(short))));
+typedef __attribute__((address_space(3))) s4v_t lds_s4v_t;
+
+// Loads of 16 keys of one KV head (one page holds them: page sizes are
+// multiples of 16) straight into LDS, their 16-byte chunks swizzled by row.
+template <int HD>
+struct PageLoads {
+  static constexpr int kLanes = HD / 8;             // lanes on a row
+  static constexpr int kN = 16 * HD * 2 / 1024;     // load instructions
+  const uint8_t *k, *v;                             // the head's first row in page 0
+  uint32_t page_bytes, pages, mask;
+  uint32_t off[kN];                                 // the lane's byte offsets among the 16 rows
+
+  __device__ __forceinline__ PageLoads(const PagedAttn& a, int kvh, int lane) {
+    const uint32_t head = (uint32_t)(HD * 2) << a.ps_log2;  // bytes of a head's rows of a page
+    page_bytes = head * (uint32_t)a.nkv;
+    pages = (uint32_t)a.num_pages;
+    mask = (1u << a.ps_log2) - 1;
+    k = (const uint8_t*)a.k_pool + (uint64_t)head * (uint32_t)kvh;
+    v = (const uint8_t*)a.v_pool + (uint64_t)head * (uint32_t)kvh;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) off[i] = (uint32_t)((i * (64 / kLanes) + lane / kLanes) * (HD * 2)) + chunk(lane, i);
+  }
+  __device__ __forceinline__ static uint32_t chunk(int lane, int i) {
+    return (uint32_t)(((lane % kLanes) ^ swizzle<HD>(i * (64 / kLanes) + lane / kLanes)) << 4);
+  }
+  // keys key .. key + 15 (those outside [lo, hi) as the nearest inside) to LDS at dst
+  __device__ __forceinline__ void issue(const uint8_t* base, int page, int key, int lo, int hi, uint32_t dst, int lane,
+                                        bool& bad) const {
+    const bool ok = (uint32_t)page < pages;
+    bad = bad || !ok;
+    const uint8_t* src = base + (uint64_t)(ok ? (uint32_t)page : 0u) * page_bytes + ((uint32_t)key & mask) * (HD * 2);
+    if (key >= lo && key + 16 <= hi) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) lds_dma16(src, off[i], dst + i * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const int r = min(max(i * (64 / kLanes) + lane / kLanes, lo - key), hi - 1 - key);
+        lds_dma16(src, (uint32_t)(r * (HD * 2)) + chunk(lane, i), dst + i * 1024);
+      }
+    }
+  }
+};
+
 // The keys of an item: `pre_steps` steps of the prefix's `pre` keys (none: 0),
 // then the steps of a sequence's own keys [0, hi), P of them cached and new rows
 // after those. Keys are counted in 32 bits: a sequence is shorter than 2^30.
@@ -161,43 +206,29 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
   const const_i32 tab_own = (const_i32)(uintptr_t)uniform_ptr((const uint16_t*)k.table);
   const int psl = a.ps_log2;
   const int lo_pre = min(k.lo, max(k.pre - 1, 0)), lo_own = min(max(k.lo - k.base, 0), max(k.hi - 1, 0));
-  // the pages of this wave's pieces of a step, asked for a step ahead
-  int page[C::kChunks];
-  auto piece_of = [&](int step, int c) {  // its 16 keys' index in the step's list
-    const bool pre = step < k.pre_steps;
-    const int ch = (wave * C::kChunks + c) % (C::SK / 16);
-    const int p = (pre ? step : step - k.pre_steps) * (C::SK / 16) + ch;
-    return max((pre ? lo_pre : lo_own) >> 4, min(p, ((pre ? k.pre : k.hi) - 1) >> 4));
-  };
+  const PageLoads<HD> ld(a, kvh, lane);
+  // this wave's pieces (16 keys of K or V) of a step: the keys and their page, asked for a step ahead
+  int page[C::kChunks], key[C::kChunks];
   auto ask = [&](int step) {
-    const const_i32 tab = step < k.pre_steps ? tab_pre : tab_own;
-#pragma unroll
-    for (int c = 0; c < C::kChunks; ++c) page[c] = tab[(piece_of(step, c) << 4) >> psl];
-  };
-  auto issue = [&](int step) {
-    const uint32_t buf = lds_base + (step % C::ST) * C::kStep;
     const bool pre = step < k.pre_steps;
+    const const_i32 tab = pre ? tab_pre : tab_own;
+    const int at = (pre ? step : step - k.pre_steps) * C::SK;
+    const int first = (pre ? lo_pre : lo_own) & ~15, last = ((pre ? k.pre : k.hi) - 1) & ~15;
 #pragma unroll
     for (int c = 0; c < C::kChunks; ++c) {
-      const int piece = wave * C::kChunks + c, ch = piece % (C::SK / 16);
-      const bool is_v = piece >= C::SK / 16;
-      const int k16 = piece_of(step, c) << 4;
-      int pgid = page[c];
-      if (pgid < 0 || pgid >= a.num_pages) {
-        bad = true;
-        pgid = 0;
-      }
-      const int64_t row = (((int64_t)pgid * a.nkv + kvh) << psl) + (k16 & ((1 << psl) - 1));
-      const uint16_t* src = uniform_ptr((const uint16_t*)(is_v ? a.v_pool : a.k_pool) + row * HD);
-      const uint32_t dst = __builtin_amdgcn_readfirstlane(buf + (is_v ? C::kHalf : 0) + ch * 16 * HD * 2);
-      const int rlo = max((pre ? lo_pre : lo_own) - k16, 0), rhi = min((pre ? k.pre : k.hi) - 1 - k16, 15);
+      key[c] = max(first, min(at + 16 * ((wave * C::kChunks + c) % (C::SK / 16)), last));
+      page[c] = tab[key[c] >> psl];
+    }
+  };
+  auto issue = [&](int step) {
+    const bool pre = step < k.pre_steps;
+    const uint32_t buf = lds_base + (step % C::ST) * C::kStep;
 #pragma unroll
-      for (int i = 0; i < C::kPerChunk; ++i) {
-        constexpr int kLanes = HD / 8;  // lanes on a row
-        const int r = i * (64 / kLanes) + lane / kLanes;
-        const int rr = min(max(r, rlo), rhi);
-        lds_dma16(src, (uint32_t)(rr * (HD * 2) + (((lane % kLanes) ^ swizzle<HD>(r)) << 4)), dst + i * 1024);
-      }
+    for (int c = 0; c < C::kChunks; ++c) {
+      const int piece = wave * C::kChunks + c;
+      const bool is_v = piece >= C::SK / 16;
+      ld.issue(is_v ? ld.v : ld.k, page[c], key[c], pre ? lo_pre : lo_own, pre ? k.pre : k.hi,
+               buf + (is_v ? C::kHalf : 0) + (piece % (C::SK / 16)) * 16 * HD * 2, lane, bad);
     }
   };
 
@@ -211,8 +242,18 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
   const bool tree = a.mask_mode == PE_MASK_TREE;
   const float cap_in = MOD && a.softcap > 0.f ? 2.f * scale2 / a.softcap : 0.f, cap_out = a.softcap * kLog2e;
 
+  // the lane's LDS offsets: K row ln of a 32-key block, and V's transposed reads
+  const int qg = lane >> 4, jl = lane & 15, vrow = 4 * (qg >> 1) + (jl >> 2), vcol = 16 * (qg & 1) + 4 * (jl & 3);
+  uint32_t k_at[HD / 16], v_at[2][OB];
+#pragma unroll
+  for (int j = 0; j < HD / 16; ++j) k_at[j] = lds_at<HD>(ln, 2 * j + g);
+#pragma unroll
+  for (int h = 0; h < OB; ++h)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) v_at[e][h] = lds_at<HD>(vrow + 8 * e, (32 * (hb + h) + vcol) >> 3) + (vcol & 7) * 2;
+
   if (s0 < s1) ask(s0);
-  __syncthreads();  // the buffers' and hand-over's last readers are done
+  __syncthreads();  // the buffers' last readers are done
 #pragma unroll
   for (int i = 0; i < C::ST - 1; ++i)
     if (s0 + i < s1) {
@@ -236,15 +277,46 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
     const uint8_t* kbp = smem + (s % C::ST) * C::kStep;
     const uint8_t* vbp = kbp + C::kHalf;
     f32x16_t sc[SB];
+    // Fragments in groups of LDS reads, kAhead groups ahead of the products that
+    // use them: kS groups of four products of S, then 2 SB groups (16 keys each)
+    // of V, whose first kAhead are read before the softmax. (One group ahead
+    // where the other scores' registers leave no room: two spilled 38.)
+    constexpr int kS = SB * HD / 64, kAll = kS + 2 * SB, kAhead = MOD && HD == 128 ? 1 : 2, kF = kAhead + 1;
+    u32x4_t f[kF][4];
+    auto read = [&](int gr) {
+      if (gr < kS) {
 #pragma unroll
-    for (int sb = 0; sb < SB; ++sb)
+        for (int i = 0; i < 4; ++i) {
+          const int at = 4 * gr + i;  // product SB j + sb
+          f[gr % kF][i] = *(const u32x4_t*)(kbp + k_at[at / SB] + (at % SB) * 32 * HD * 2);
+        }
+      } else if (gr < kAll) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sc[sb][i] = 0.f;
+        for (int h = 0; h < OB; ++h) {
+          const uint8_t* vq = vbp + (gr - kS) * 16 * HD * 2;
+          const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v_t*)(vq + v_at[0][h])));
+          const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v_t*)(vq + v_at[1][h])));
+          f[gr % kF][h] = u32x4_t{x.x, x.y, y.x, y.y};
+        }
+      }
+    };
 #pragma unroll
-    for (int j = 0; j < HD / 16; ++j)
+    for (int gr = 0; gr < kAhead; ++gr) read(gr);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int sb = 0; sb < SB; ++sb)
-        sc[sb] = mfma32<DT>(*(const u32x4_t*)(kbp + lds_at<HD>(32 * sb + ln, 2 * j + g)), qf[j], sc[sb]);
+    for (int gr = 0; gr < kS; ++gr) {
+      read(gr + kAhead);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = 4 * gr + i;
+        if (at < SB)
+          sc[at] = mfma32<DT>(f[gr % kF][i], qf[0], f32x16_t{});
+        else
+          sc[at % SB] = mfma32<DT>(f[gr % kF][i], qf[at / SB], sc[at % SB]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
     // sc[sb][i] is key kb0 + 32 sb + 8 (i / 4) + 4 g + i % 4 of the lane's row
     const bool node_step = !pre && kb0 + 32 * SB > k.P;
     if constexpr (MOD) {
@@ -332,25 +404,15 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
     }
     m = mnew;
     // O^T += V^T P^T over the 16-key quarters of the step
-    const int qg = lane >> 4, jl = lane & 15;
 #pragma unroll
     for (int c = 0; c < 2 * SB; ++c) {
-      const int sb = c >> 1, cq = c & 1;
-      const u32x4_t bp = {pb[sb][4 * cq], pb[sb][4 * cq + 1], pb[sb][4 * cq + 2], pb[sb][4 * cq + 3]};
-      const int kb = 16 * c + 4 * (qg >> 1) + (jl >> 2);
+      const int q = c & 1;
+      const u32x4_t bp = {pb[c >> 1][4 * q], pb[c >> 1][4 * q + 1], pb[c >> 1][4 * q + 2], pb[c >> 1][4 * q + 3]};
+      read(kS + c + kAhead);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int h = 0; h < OB; ++h) {
-        const int db = 32 * (hb + h) + 16 * (qg & 1) + 4 * (jl & 3);
-        typedef short s4v_t __attribute__((__vector_size__(4 * sizeof(short))));
-        typedef __attribute__((address_space(3))) s4v_t lds_s4v_t;
-        const uint2 lo = __builtin_bit_cast(
-            uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v_t*)(vbp + lds_at<HD>(kb, db >> 3) + (db & 7) * 2)));
-        const uint2 hi = __builtin_bit_cast(
-            uint2,
-            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v_t*)(vbp + lds_at<HD>(kb + 8, db >> 3) + (db & 7) * 2)));
-        const u32x4_t av = {lo.x, lo.y, hi.x, hi.y};
-        o[h] = mfma32<DT>(av, bp, o[h]);
-      }
+      for (int h = 0; h < OB; ++h) o[h] = mfma32<DT>(f[(kS + c) % kF][h], bp, o[h]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   l = sum_halves(l);
@@ -395,28 +457,16 @@ __device__ __forceinline__ void attend_wide(const PagedAttn& a, uint8_t* smem, c
   typedef const __attribute__((address_space(4))) int32_t* const_i32;
   const const_i32 tab = (const_i32)(uintptr_t)uniform_ptr((const uint16_t*)table);
   const int psl = a.ps_log2, lo_k = min(lo, n - 1);
+  const PageLoads<HD> ld(a, kvh, lane);
   const int ch = wave & 3;  // this wave's 16 keys of K (waves 0 - 3) or V of a step
-  const uint16_t* pool = (const uint16_t*)(grp ? a.v_pool : a.k_pool);
-  int page = 0;
-  auto piece_of = [&](int step) { return max(lo_k >> 4, min(step * 4 + ch, (n - 1) >> 4)); };
-  auto ask = [&](int step) { page = tab[(piece_of(step) << 4) >> psl]; };
+  int page = 0, key = 0;
+  auto ask = [&](int step) {
+    key = max(lo_k & ~15, min(step * 64 + 16 * ch, (n - 1) & ~15));
+    page = tab[key >> psl];
+  };
   auto issue = [&](int step) {
-    const int k16 = piece_of(step) << 4;
-    int pgid = page;
-    if (pgid < 0 || pgid >= a.num_pages) {
-      bad = true;
-      pgid = 0;
-    }
-    const int64_t row = (((int64_t)pgid * a.nkv + kvh) << psl) + (k16 & ((1 << psl) - 1));
-    const uint16_t* src = uniform_ptr(pool + row * HD);
-    const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_base + (step & 3) * C::kStep + grp * C::kHalf + ch * 16 * HD * 2);
-    const int rlo = max(lo_k - k16, 0), rhi = min(n - 1 - k16, 15);
-#pragma unroll
-    for (int i = 0; i < C::kPerChunk; ++i) {
-      constexpr int kLanes = HD / 8;
-      const int r = i * (64 / kLanes) + lane / kLanes;
-      lds_dma16(src, (uint32_t)(min(max(r, rlo), rhi) * (HD * 2) + (((lane % kLanes) ^ swizzle<HD>(r)) << 4)), dst + i * 1024);
-    }
+    ld.issue(grp ? ld.v : ld.k, page, key, lo_k, n, lds_base + (step & 3) * C::kStep + grp * C::kHalf + ch * 16 * HD * 2,
+             lane, bad);
   };
 
 #pragma unroll
@@ -446,8 +496,6 @@ __device__ __forceinline__ void attend_wide(const PagedAttn& a, uint8_t* smem, c
     v_at[0][h] = lds_at<HD>(vrow, (32 * h + vcol) >> 3) + (vcol & 7) * 2;
     v_at[1][h] = lds_at<HD>(vrow + 8, (32 * h + vcol) >> 3) + (vcol & 7) * 2;
   }
-  typedef short s4v_t __attribute__((__vector_size__(4 * sizeof(short))));
-  typedef __attribute__((address_space(3))) s4v_t lds_s4v_t;
 
   // Phase X: `pv`: step s - 1's P V, `qk`: step s's scores. Groups of LDS reads
   // 0 .. 3: V of a 16-key quarter (4 products of hd 128, 2 of 64), then K, as

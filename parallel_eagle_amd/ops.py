@@ -397,39 +397,37 @@ def kv_gather(k_cache, v_cache, keep: torch.Tensor, status4: torch.Tensor) -> No
 
 
 # ------------------------------------------------------------------ paged cache
-def _same_device(*tensors) -> torch.device:
-    """The device of a call's tensors (None entries skipped)."""
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("parallel_eagle_amd kernels take HIP device tensors")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"tensors of one call on {dev} and {t.device}")
-    return dev
+def _call_on(index: int, fn, *args) -> int:
+    """fn(*args, stream) on the current stream of device ``index``, whatever the current device is."""
+    if index == torch._C._cuda_getDevice():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _call_on(dev: torch.device, fn, *args) -> int:
-    """fn(*args, stream) on dev's current stream, whatever the current device is."""
-    cur = torch.cuda.current_device()
-    if dev.index == cur:
-        return fn(*args, torch._C._cuda_getCurrentRawStream(cur))
-    with torch.cuda.device(dev):
-        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+def _device_index(t: torch.Tensor) -> int:
+    if not t.is_cuda:
+        raise ValueError("parallel_eagle_amd kernels take HIP device tensors")
+    return t.get_device()
 
 
-def _req_vec(t: torch.Tensor, dtype: torch.dtype, n: int, name: str) -> None:
-    if t.dtype != dtype or t.dim() != 1 or t.numel() < n or (t.numel() > 1 and t.stride(0) != 1):
-        raise ValueError(f"{name} must be contiguous {dtype} with at least {n} elements")
+def _vec(t: torch.Tensor, dtype: torch.dtype, n: int, dev: int, name: str) -> int:
+    """The pointer of a contiguous vector of at least n elements on device ``dev``."""
+    if t.dtype is not dtype or t.get_device() != dev or t.numel() < n or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {dtype} with at least {n} elements, on the device of the call's "
+                         "other tensors")
+    return t.data_ptr()
 
 
-def _req_table(table: torch.Tensor, batch: int) -> None:
-    if (table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] < batch or table.shape[1] < 1
-            or table.stride(1) != 1 or table.stride(0) < table.shape[1]):
-        raise ValueError("block_table must be int32 [batch][pages] with contiguous rows, one per sequence")
+def _table(t: torch.Tensor, batch: int, dev: int) -> tuple[int, int, int]:
+    """Pointer, entries between two rows and entries of a row of a block table."""
+    if t.dtype is not torch.int32 or t.get_device() != dev or t.dim() != 2:
+        raise ValueError("block_table must be int32 [batch][pages] on the device of the call's other tensors")
+    rows, cols = t.shape
+    ld, unit = t.stride()
+    if rows < batch or cols < 1 or (unit != 1 and cols > 1) or (rows > 1 and ld < cols):
+        raise ValueError("block_table must have contiguous rows, one per sequence")
+    return t.data_ptr(), ld if rows > 1 else cols, cols
 
 
 def page_tables(seq_len: torch.Tensor, seq_row0: torch.Tensor, block_table: torch.Tensor, held: torch.Tensor,
@@ -445,56 +443,55 @@ def page_tables(seq_len: torch.Tensor, seq_row0: torch.Tensor, block_table: torc
     and ``free_top`` are updated in place unless ``held_out`` / ``top_out``
     receive the new counts. Slot -1: a row behind the last sequence, or without a
     page (PE_ERR_CAPACITY in ``status``)."""
-    dev = _same_device(seq_len, seq_row0, block_table, held, free_pages, free_top, status, held_out, top_out, slots)
+    dev = _device_index(seq_row0)
     b = seq_row0.numel() - 1
-    _req(b >= 1 and 0 <= rows < 2 ** 31, "seq_row0 must hold batch + 1 offsets, rows must be a count")
-    _req_vec(seq_row0, torch.int32, b + 1, "seq_row0")
-    _req_vec(seq_len, torch.int64, b, "seq_len")
-    _req_table(block_table, b)
-    _req_vec(held, torch.int32, b, "held")
-    _req_vec(free_pages, torch.int32, 0, "free_pages")
-    _req_vec(free_top, torch.int32, 1, "free_top")
-    _req_vec(status, torch.int32, 1, "status")
-    held_out, top_out = held if held_out is None else held_out, free_top if top_out is None else top_out
-    _req_vec(held_out, torch.int32, b, "held_out")
-    _req_vec(top_out, torch.int32, 1, "top_out")
+    if b < 1 or not 0 <= rows < 2 ** 31:
+        raise ValueError("seq_row0 must hold batch + 1 offsets, rows must be a count")
+    i32 = torch.int32
+    p_row0, p_len = _vec(seq_row0, i32, b + 1, dev, "seq_row0"), _vec(seq_len, torch.int64, b, dev, "seq_len")
+    p_tab, ld, cols = _table(block_table, b, dev)
+    p_held, p_top = _vec(held, i32, b, dev, "held"), _vec(free_top, i32, 1, dev, "free_top")
+    p_free, p_status = _vec(free_pages, i32, 0, dev, "free_pages"), _vec(status, i32, 1, dev, "status")
+    o_held = p_held if held_out is None else _vec(held_out, i32, b, dev, "held_out")
+    o_top = p_top if top_out is None else _vec(top_out, i32, 1, dev, "top_out")
     if slots is None:
-        slots = torch.empty(rows, dtype=torch.int64, device=dev)
-    _req_vec(slots, torch.int64, rows, "slots")
-    hp, tp = held.data_ptr(), free_top.data_ptr()
+        slots = torch.empty(rows, dtype=torch.int64, device=seq_row0.device)
+    p_slots = _vec(slots, torch.int64, rows, dev, "slots")
     scratch = None
-    if held_out.data_ptr() == hp or top_out.data_ptr() == tp:
-        scratch = torch.empty(b + 1, dtype=torch.int32, device=dev)
-    check(_call_on(dev, lib().pe_page_tables, seq_len.data_ptr(), seq_row0.data_ptr(), b, rows, prefix_len, page_size,
-                   block_table.data_ptr(), block_table.stride(0), block_table.shape[1], hp, free_pages.data_ptr(),
-                   free_pages.numel(), tp, held_out.data_ptr(), top_out.data_ptr(),
-                   None if scratch is None else scratch.data_ptr(), slots.data_ptr(), status.data_ptr()),
-          "pe_page_tables")
-    return slots[:rows]
+    if o_held == p_held or o_top == p_top:
+        scratch = torch.empty(b + 1, dtype=i32, device=seq_row0.device)
+    check(_call_on(dev, lib().pe_page_tables, p_len, p_row0, b, rows, prefix_len, page_size, p_tab, ld, cols, p_held,
+                   p_free, free_pages.numel(), p_top, o_held, o_top, None if scratch is None else scratch.data_ptr(),
+                   p_slots, p_status), "pe_page_tables")
+    return slots if slots.numel() == rows else slots[:rows]
 
 
 def page_release(seqs: torch.Tensor, block_table: torch.Tensor, held: torch.Tensor, free_pages: torch.Tensor,
                  free_top: torch.Tensor, status: torch.Tensor) -> None:
     """Return the pages of the listed sequences (int32, each once) to the free list (pe_page_release)."""
-    dev = _same_device(seqs, block_table, held, free_pages, free_top, status)
+    dev = _device_index(held)
     b = held.numel()
-    _req_vec(seqs, torch.int32, 0, "seqs")
-    _req(b >= 1, "held must name the sequences")
-    _req_vec(held, torch.int32, b, "held")
-    _req_table(block_table, b)
-    _req_vec(free_pages, torch.int32, 1, "free_pages")
-    _req_vec(free_top, torch.int32, 1, "free_top")
-    _req_vec(status, torch.int32, 1, "status")
-    check(_call_on(dev, lib().pe_page_release, seqs.data_ptr(), seqs.numel(), b, block_table.data_ptr(),
-                   block_table.stride(0), block_table.shape[1], held.data_ptr(), free_pages.data_ptr(),
-                   free_pages.numel(), free_top.data_ptr(), status.data_ptr()), "pe_page_release")
+    if b < 1:
+        raise ValueError("held must name the sequences")
+    i32 = torch.int32
+    p_tab, ld, cols = _table(block_table, b, dev)
+    check(_call_on(dev, lib().pe_page_release, _vec(seqs, i32, 0, dev, "seqs"), seqs.numel(), b, p_tab, ld, cols,
+                   _vec(held, i32, b, dev, "held"), _vec(free_pages, i32, 1, dev, "free_pages"), free_pages.numel(),
+                   _vec(free_top, i32, 1, dev, "free_top"), _vec(status, i32, 1, dev, "status")), "pe_page_release")
 
 
-def _req_pools(k_pool: torch.Tensor, v_pool: torch.Tensor, dim: int) -> None:
-    if (k_pool.dim() != dim or k_pool.shape != v_pool.shape or k_pool.dtype != v_pool.dtype
-            or not k_pool.is_contiguous() or not v_pool.is_contiguous() or k_pool.numel() == 0):
+def _pools(k_pool: torch.Tensor, v_pool: torch.Tensor, dim: int, dev: int) -> tuple:
+    """The shape of a pair of pools."""
+    shape = k_pool.shape
+    if (len(shape) != dim or v_pool.shape != shape or k_pool.dtype is not v_pool.dtype or k_pool.get_device() != dev
+            or v_pool.get_device() != dev or not k_pool.is_contiguous() or not v_pool.is_contiguous()
+            or k_pool.numel() == 0):
         raise ValueError(f"pools must be contiguous {'[L]' if dim == 5 else ''}[pages][nkv][page_size][hd], K and V "
-                         "alike")
+                         "alike, on the device of the call's other tensors")
+    return shape
+
+
+_I64x3 = C.c_int64 * 3
 
 
 def kv_write_paged(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, slots: torch.Tensor,
@@ -503,39 +500,39 @@ def kv_write_paged(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_poo
     cache's rows, or columns of a fused q/k/v block) to their slots of the pools
     [L][pages][nkv][page_size][hd] (pe_kv_write_paged). Rows of slot -1 are
     skipped; slots are distinct."""
-    dev = _same_device(k, v, k_pool, v_pool, slots, status)
-    _req_pools(k_pool, v_pool, 5)
-    L, pages, nkv, ps, hd = k_pool.shape
-    _req(k.dim() == 4 and k.shape == v.shape and k.shape[0] == L and k.shape[2:] == (nkv, hd)
-         and k.dtype == v.dtype == k_pool.dtype and (hd == 1 or (k.stride(3) == 1 and v.stride(3) == 1)),
-         "k and v must be [L][M][nkv][hd] in the pools' layers, heads and dtype with contiguous head rows")
-    m = k.shape[1]
-    _req_vec(slots, torch.int64, m, "slots")
-    _req(slots.numel() == m, "one slot per row")
-    _req_vec(status, torch.int32, 1, "status")
-    s3 = C.c_int64 * 3
-    check(_call_on(dev, lib().pe_kv_write_paged, k.data_ptr(), v.data_ptr(), s3(*k.stride()[:3]), s3(*v.stride()[:3]),
-                   L, m, nkv, hd, dcode(k_pool.dtype), k_pool.data_ptr(), v_pool.data_ptr(), pages, ps,
-                   slots.data_ptr(), status.data_ptr()), "pe_kv_write_paged")
+    dev = _device_index(slots)
+    L, pages, nkv, ps, hd = _pools(k_pool, v_pool, 5, dev)
+    dt = k_pool.dtype
+    shape, ks, vs = k.shape, k.stride(), v.stride()
+    if (len(shape) != 4 or v.shape != shape or shape[0] != L or shape[2] != nkv or shape[3] != hd or k.dtype is not dt
+            or v.dtype is not dt or (hd > 1 and (ks[3] != 1 or vs[3] != 1)) or k.get_device() != dev
+            or v.get_device() != dev):
+        raise ValueError("k and v must be [L][M][nkv][hd] in the pools' layers, heads, dtype and device with contiguous "
+                         "head rows")
+    m = shape[1]
+    p_slots = _vec(slots, torch.int64, m, dev, "slots")
+    if slots.numel() != m:
+        raise ValueError("one slot per row")
+    check(_call_on(dev, lib().pe_kv_write_paged, k.data_ptr(), v.data_ptr(), _I64x3(*ks[:3]), _I64x3(*vs[:3]), L, m, nkv,
+                   hd, dcode(dt), k_pool.data_ptr(), v_pool.data_ptr(), pages, ps, p_slots,
+                   _vec(status, torch.int32, 1, dev, "status")), "pe_kv_write_paged")
 
 
 def kv_compact_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor, seq_len: torch.Tensor,
                      accept_out: torch.Tensor, status: torch.Tensor, *, prefix_len: int = 0) -> None:
     """Every sequence's accepted rows moved together in the pools [L][pages][nkv][page_size][hd], the paths from
     ``accept_out`` int32 [B][2 + max_rows] (pe_kv_compact_paged)."""
-    dev = _same_device(k_pool, v_pool, block_table, seq_len, accept_out, status)
-    _req_pools(k_pool, v_pool, 5)
-    L, pages, nkv, ps, hd = k_pool.shape
-    _req(accept_out.dtype == torch.int32 and accept_out.dim() == 2 and accept_out.is_contiguous()
-         and accept_out.shape[1] >= 3 and accept_out.shape[0] >= 1, "accept_out must be contiguous int32 [B][2 + max_rows]")
-    b = accept_out.shape[0]
-    _req_table(block_table, b)
-    _req_vec(seq_len, torch.int64, b, "seq_len")
-    _req_vec(status, torch.int32, 1, "status")
+    dev = _device_index(accept_out)
+    L, pages, nkv, ps, hd = _pools(k_pool, v_pool, 5, dev)
+    if (accept_out.dtype is not torch.int32 or accept_out.dim() != 2 or not accept_out.is_contiguous()
+            or accept_out.shape[1] < 3 or accept_out.shape[0] < 1):
+        raise ValueError("accept_out must be contiguous int32 [B][2 + max_rows]")
+    b, width = accept_out.shape
+    p_tab, ld, cols = _table(block_table, b, dev)
     check(_call_on(dev, lib().pe_kv_compact_paged, k_pool.data_ptr(), v_pool.data_ptr(), L, nkv, hd,
-                   dcode(k_pool.dtype), pages, ps, block_table.data_ptr(), block_table.stride(0),
-                   block_table.shape[1], b, seq_len.data_ptr(), prefix_len, accept_out.data_ptr(),
-                   accept_out.shape[1] - 2, status.data_ptr()), "pe_kv_compact_paged")
+                   dcode(k_pool.dtype), pages, ps, p_tab, ld, cols, b, _vec(seq_len, torch.int64, b, dev, "seq_len"),
+                   prefix_len, accept_out.data_ptr(), width - 2, _vec(status, torch.int32, 1, dev, "status")),
+          "pe_kv_compact_paged")
 
 
 def attention_paged_workspace_bytes(m: int, batch: int, nh: int, nkv: int, hd: int, max_rows: int, max_len: int,
@@ -562,54 +559,56 @@ def tree_attention_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     scores by a tanh, ``slopes`` fp32 [nh] subtracts slope * distance, ``window``
     hides keys that far back: the last two need ``positions`` int64 [M]. Rows of
     no sequence are left as they are in ``out``."""
-    dev = _same_device(q, k_pool, v_pool, block_table, seq_row0, seq_len, status, bits, positions, prefix_table, slopes,
-                       workspace, out)
-    _req(q.dim() == 3 and q.dtype == k_pool.dtype, "q must be [M][nh][hd] in the pools' dtype")
-    m, nh, hd = q.shape
-    _req_pools(k_pool, v_pool, 4)
-    pages, nkv, ps, phd = k_pool.shape
-    _req(phd == hd and (hd == 1 or q.stride(2) == 1) and (nh == 1 or q.stride(1) == hd)
-         and (m <= 1 or q.stride(0) >= nh * hd), "q rows must hold their heads one after another, as wide as the pools'")
+    dev = _device_index(q)
+    shape, dt = q.shape, q.dtype
+    if len(shape) != 3 or k_pool.dtype is not dt:
+        raise ValueError("q must be [M][nh][hd] in the pools' dtype")
+    m, nh, hd = shape
+    pages, nkv, ps, phd = _pools(k_pool, v_pool, 4, dev)
+    ld_q, s_head, s_dim = q.stride()
+    if phd != hd or (hd > 1 and s_dim != 1) or (nh > 1 and s_head != hd) or (m > 1 and ld_q < nh * hd):
+        raise ValueError("q rows must hold their heads one after another, as wide as the pools'")
     b = seq_row0.numel() - 1
-    _req(b >= 1, "seq_row0 must hold batch + 1 offsets")
-    _req_vec(seq_row0, torch.int32, b + 1, "seq_row0")
-    _req_vec(seq_len, torch.int64, b, "seq_len")
-    _req_table(block_table, b)
-    _req_vec(status, torch.int32, 1, "status")
-    words = 0
+    if b < 1:
+        raise ValueError("seq_row0 must hold batch + 1 offsets")
+    p_row0, p_len = _vec(seq_row0, torch.int32, b + 1, dev, "seq_row0"), _vec(seq_len, torch.int64, b, dev, "seq_len")
+    p_tab, ld, cols = _table(block_table, b, dev)
+    p_status = _vec(status, torch.int32, 1, dev, "status")
+    p_bits = p_pos = p_slopes = p_pre = None
+    words = n_pre = 0
     if mask_mode == _lib.PE_MASK_TREE:
-        _req(bits is not None and bits.dtype == torch.int64 and bits.dim() == 2 and bits.shape[0] >= m
-             and bits.is_contiguous(), "tree masks need contiguous int64 bits [M][words]")
-        words = bits.shape[1]
+        if (bits is None or bits.dtype is not torch.int64 or bits.dim() != 2 or bits.shape[0] < m
+                or not bits.is_contiguous() or bits.get_device() != dev):
+            raise ValueError("tree masks need contiguous int64 bits [M][words] on the device of the call's other tensors")
+        p_bits, words = bits.data_ptr(), bits.shape[1]
     if window or slopes is not None:
-        _req(positions is not None, "a window or slopes need positions")
-    if positions is not None:
-        _req_vec(positions, torch.int64, m, "positions")
+        if positions is None:
+            raise ValueError("a window or slopes need positions")
+        p_pos = _vec(positions, torch.int64, m, dev, "positions")
     if slopes is not None:
-        _req_vec(slopes, torch.float32, nh, "slopes")
+        p_slopes = _vec(slopes, torch.float32, nh, dev, "slopes")
     if prefix_len:
-        _req(prefix_table is not None, "a prefix needs its pages")
-        _req_vec(prefix_table, torch.int32, 1, "prefix_table")
+        if prefix_table is None:
+            raise ValueError("a prefix needs its pages")
+        p_pre, n_pre = _vec(prefix_table, torch.int32, 1, dev, "prefix_table"), prefix_table.numel()
     if out is None:
-        out = torch.empty((m, nh * hd), dtype=q.dtype, device=dev)
-    _req(out.shape == (m, nh * hd) and out.dtype == q.dtype and (out.stride(1) == 1 or nh * hd == 1)
-         and (m <= 1 or out.stride(0) >= nh * hd), "out must be [M][nh * hd] in q's dtype with contiguous rows")
-    need = attention_paged_workspace_bytes(m, b, nh, nkv, hd, max_rows, max_len, prefix_len, q.dtype)
-    if workspace is None and need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    ws_bytes = 0
+        out = torch.empty((m, nh * hd), dtype=dt, device=q.device)
+    elif (out.shape != (m, nh * hd) or out.dtype is not dt or out.get_device() != dev
+          or (nh * hd > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < nh * hd)):
+        raise ValueError("out must be [M][nh * hd] in q's dtype and device with contiguous rows")
+    if workspace is None:
+        need = attention_paged_workspace_bytes(m, b, nh, nkv, hd, max_rows, max_len, prefix_len, dt)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    p_ws, ws_bytes = None, 0
     if workspace is not None:
-        _req(workspace.is_contiguous(), "workspace must be contiguous")
-        ws_bytes = workspace.numel() * workspace.element_size()
+        if not workspace.is_contiguous() or workspace.get_device() != dev:
+            raise ValueError("workspace must be contiguous, on the device of the call's other tensors")
+        p_ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     a = _lib.PagedAttentionArgs(
-        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), block_table.data_ptr(),
-        prefix_table.data_ptr() if prefix_len else None, seq_row0.data_ptr(), seq_len.data_ptr(),
-        bits.data_ptr() if words else None, None if positions is None else positions.data_ptr(),
-        None if slopes is None else slopes.data_ptr(), None if workspace is None else workspace.data_ptr(),
-        status.data_ptr(), ws_bytes, q.stride(0) if m > 1 else nh * hd, out.stride(0) if m > 1 else nh * hd,
-        block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1], block_table.shape[1], pages,
-        prefix_table.numel() if prefix_len else 0, prefix_len, max_len, window, m, b, max_rows, nh, nkv, hd, ps,
-        dcode(q.dtype), mask_mode, words, scale, softcap, 0)
+        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), p_tab, p_pre, p_row0, p_len, p_bits, p_pos,
+        p_slopes, p_ws, p_status, ws_bytes, ld_q if m > 1 else nh * hd, out.stride(0) if m > 1 else nh * hd, ld, cols,
+        pages, n_pre, prefix_len, max_len, window, m, b, max_rows, nh, nkv, hd, ps, dcode(dt), mask_mode, words, scale,
+        softcap, 0)
     check(_call_on(dev, lib().pe_tree_attention_paged, C.byref(a)), "pe_tree_attention_paged")
     return out
 
