@@ -276,12 +276,13 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
     if (!live || (!pre && kb0 > k.last)) continue;  // wave-uniform: the tile sees no key of this step
     const uint8_t* kbp = smem + (s % C::ST) * C::kStep;
     const uint8_t* vbp = kbp + C::kHalf;
-    f32x16_t sc[SB];
+    // products on two chains of accumulators at least (a chain alone waits for each product)
+    constexpr int kChains = SB > 1 ? SB : 2;
+    f32x16_t sc[kChains];
     // Fragments in groups of LDS reads, kAhead groups ahead of the products that
     // use them: kS groups of four products of S, then 2 SB groups (16 keys each)
-    // of V, whose first kAhead are read before the softmax. (One group ahead
-    // where the other scores' registers leave no room: two spilled 38.)
-    constexpr int kS = SB * HD / 64, kAll = kS + 2 * SB, kAhead = MOD && HD == 128 ? 1 : 2, kF = kAhead + 1;
+    // of V, whose first kAhead are read before the softmax.
+    constexpr int kS = SB * HD / 64, kAll = kS + 2 * SB, kAhead = 2, kF = kAhead + 1;
     u32x4_t f[kF][4];
     auto read = [&](int gr) {
       if (gr < kS) {
@@ -310,12 +311,14 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int at = 4 * gr + i;
-        if (at < SB)
-          sc[at] = mfma32<DT>(f[gr % kF][i], qf[0], f32x16_t{});
-        else
-          sc[at % SB] = mfma32<DT>(f[gr % kF][i], qf[at / SB], sc[at % SB]);
+        sc[at % kChains] =
+            mfma32<DT>(f[gr % kF][i], qf[at / SB], at < kChains ? f32x16_t{} : sc[at % kChains]);
       }
       __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (SB == 1) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[0][i] += sc[1][i];
     }
     // sc[sb][i] is key kb0 + 32 sb + 8 (i / 4) + 4 g + i % 4 of the lane's row
     const bool node_step = !pre && kb0 + 32 * SB > k.P;
@@ -344,6 +347,7 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
             const int dist = u < 0 ? d0 - off : ri.pos - np;
             sc[sb][i] = fmaf(sc[sb][i], mul, -ri.slope2 * (float)dist);
             if (a.window > 0) sc[sb][i] = dist < a.window ? sc[sb][i] : -INFINITY;
+            if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // few positions in registers at a time
           }
       } else if (sloped) {
         const float c0 = -ri.slope2 * (float)d0;
@@ -915,8 +919,10 @@ __device__ __forceinline__ void seq_item(const PagedAttn& a, const PagedPrefix& 
 // Many rows over a long prefix: eight tiles (256 rows) on every K / V byte, one
 // workgroup per CU.
 template <int HD> using Wide = Cfg<HD, 8, 1, 2, 4>;
-// Four waves, 64 KiB of LDS (32 KiB for heads of 64), two workgroups per CU.
-template <int HD> using Four = Cfg<HD, 4, 1, 2, 2>;
+// Four waves, 64 KiB of LDS, two workgroups per CU. (Other scores of 128-dim
+// heads by 32 keys: 64 leave their registers no room, and a spilled one is
+// reloaded behind the loads in flight.)
+template <int HD, bool MOD> using Four = Cfg<HD, 4, 1, MOD && HD == 128 ? 1 : 2, HD == 128 && !MOD ? 2 : 4>;
 template <int HD> using Two = Cfg<HD, 4, 2, HD == 128 ? 1 : 2, 4>;
 template <int HD> using One = Cfg<HD, 4, HD == 128 ? 4 : 2, HD == 128 ? 1 : 2, 4>;
 
@@ -933,19 +939,19 @@ __global__ __launch_bounds__(512, 2) void paged_prefix_kernel(PagedAttn a, Paged
 template <int DT, int HD, bool MOD>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttn a, PagedPrefix pp, PagedParts parts, PagedSeqs sq,
                                                             uint32_t n_pre, int pre_kind) {
-  constexpr int kSmem = Two<HD>::kSmem > Four<HD>::kSmem ? Two<HD>::kSmem : Four<HD>::kSmem;
+  constexpr int kSmem = Two<HD>::kSmem > Four<HD, MOD>::kSmem ? Two<HD>::kSmem : Four<HD, MOD>::kSmem;
   static_assert(One<HD>::kSmem <= kSmem, "one ring for every kind");
   __shared__ __align__(1024) uint8_t smem[kSmem];
   __shared__ int s_npos[MOD ? 64 * PE_TREE_MAX_WORDS : 1];
   __shared__ int s_lo[4];
   if (blockIdx.x < n_pre) {
     const uint32_t w = xcd_item(blockIdx.x, n_pre);
-    if (pre_kind == 4) prefix_share<DT, Four<HD>, MOD>(a, pp, parts, w, smem, s_lo);
+    if (pre_kind == 4) prefix_share<DT, Four<HD, MOD>, MOD>(a, pp, parts, w, smem, s_lo);
     else if (pre_kind == 2) prefix_share<DT, Two<HD>, MOD>(a, pp, parts, w, smem, s_lo);
     else prefix_share<DT, One<HD>, MOD>(a, pp, parts, w, smem, s_lo);
   } else {
     const uint32_t item = blockIdx.x - n_pre;
-    if (sq.kind == 4) seq_item<DT, Four<HD>, MOD>(a, pp, parts, sq, item, smem, s_npos, s_lo);
+    if (sq.kind == 4) seq_item<DT, Four<HD, MOD>, MOD>(a, pp, parts, sq, item, smem, s_npos, s_lo);
     else if (sq.kind == 2) seq_item<DT, Two<HD>, MOD>(a, pp, parts, sq, item, smem, s_npos, s_lo);
     else seq_item<DT, One<HD>, MOD>(a, pp, parts, sq, item, smem, s_npos, s_lo);
   }
@@ -971,7 +977,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefi
   const float2* sml = (const float2*)parts.ml + (int64_t)kvh * parts.tiles * 32 + grow;
   const int64_t o_part = (int64_t)a.nkv * parts.tiles * (32 * HD), ml_part = (int64_t)a.nkv * parts.tiles * 32;
   float m = kPagedInitMax, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  constexpr int kAhead = 8;  // parts asked for before the first is joined
+  constexpr int kAhead = 4;  // parts asked for before the first is joined
   const int n = npre + my_splits;
   for (int i0 = 0; i0 < n; i0 += kAhead) {
     float2 ml[kAhead];
@@ -982,15 +988,20 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefi
       ml[k] = sml[p * ml_part];
       v[k] = *(const f32x4_t*)(src + p * o_part);
     }
+    float mx = m;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) mx = fmaxf(mx, ml[k].x);  // past the end: the last one again
+    const float a0 = __builtin_amdgcn_exp2f(m - mx);
+    m = mx;
+    l *= a0;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[d] *= a0;
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      if (i0 + k >= n) break;
-      const float mx = fmaxf(m, ml[k].x);
-      const float a0 = __builtin_amdgcn_exp2f(m - mx), a1 = __builtin_amdgcn_exp2f(ml[k].x - mx);
-      m = mx;
-      l = a0 * l + a1 * ml[k].y;
+      const float a1 = i0 + k < n ? __builtin_amdgcn_exp2f(ml[k].x - mx) : 0.f;
+      l = fmaf(a1, ml[k].y, l);
 #pragma unroll
-      for (int d = 0; d < 4; ++d) o[d] = a0 * o[d] + a1 * v[k][d];
+      for (int d = 0; d < 4; ++d) o[d] = fmaf(a1, v[k][d], o[d]);
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -1003,7 +1014,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefi
 
 // ------------------------------------------------------------------ plans
 constexpr int kCus = 256;
-constexpr int kSeqWgs = 1024, kMinSplit = 64, kSplitRows = 2, kPrefixSteps = 4, kFusedPre = 256, kFoldKeys = 64;
+constexpr int kSeqWgs = 1024, kSlimWgs = 2048, kMinSplit = 64, kSplitRows = 2, kPrefixSteps = 4, kFusedPre = 256, kFoldKeys = 64;
 constexpr int64_t kWideUnits = 4096;
 
 // A launch's workgroups: which configuration, row tiles per block and how many
@@ -1017,8 +1028,8 @@ Shape shape_of(int64_t tiles, int most) {
   const int each = (int)((tiles + blocks - 1) / blocks);
   return {most == 8 ? 8 : each > 2 ? 4 : each, each, blocks};
 }
-// Keys of a step: 32 for 128-dim heads with one or two tiles, else 64.
-int step_keys(const Shape& s, int hd) { return hd == 64 || s.kind >= 4 ? 64 : 32; }
+// Keys of a step (the configurations above).
+int step_keys(const Shape& s, int hd, bool mod) { return hd == 64 || s.kind == 8 || (s.kind == 4 && !mod) ? 64 : 32; }
 
 struct Plan {
   PagedPrefix pp;
@@ -1029,7 +1040,8 @@ struct Plan {
   int64_t units, items, pre_wgs, o_bytes, ml_bytes;
 };
 
-Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int64_t max_len, int64_t prefix_len) {
+Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int64_t max_len, int64_t prefix_len,
+               bool mod) {
   Plan p;
   const int G = nh / nkv;
   const int64_t tiles = (M * G + 31) / 32;
@@ -1039,7 +1051,8 @@ Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int6
   p.pt.pre_parts = p.pre_kind = 0;
   p.wide = false;
   const Shape seq = shape_of(((int64_t)max_rows * G + 31) / 32, 4);
-  const int step = step_keys(seq, hd);
+  const int step = step_keys(seq, hd, mod);
+  const int64_t own_keys = max_len - prefix_len + max_rows;
   const bool fold = prefix_len <= std::max<int64_t>(kFoldKeys, max_rows * G);
   const int64_t pre_steps = fold ? (prefix_len + step - 1) / step : 0;
   if (!fold) {
@@ -1048,14 +1061,18 @@ Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int6
     p.wide = tiles > 4 && tiles * s64 * nkv >= kWideUnits * 8;
     const Shape pre = shape_of(tiles, p.wide ? 8 : 4);
     p.pre_kind = pre.kind;
-    const int64_t steps = (prefix_len - 1) / step_keys(pre, hd) + 1, blocks = nkv * pre.blocks;
+    const int64_t steps = (prefix_len - 1) / step_keys(pre, hd, mod) + 1, blocks = nkv * pre.blocks;
     if (p.wide) {
       p.units = blocks * steps;
       const int64_t per = (p.units + kCus - 1) / kCus;
       p.pp = PagedPrefix{(uint32_t)p.units, (uint32_t)per, (uint32_t)steps, (uint32_t)pre.blocks, (uint32_t)(32 * pre.tiles)};
       p.pt.pre_parts = (int)((steps - 1) / per) + 2;
     } else {
-      const int64_t k = std::max<int64_t>(1, std::min<int64_t>(kFusedPre / blocks, steps / kPrefixSteps));
+      // the sequences' steps of 64 keys per place, half of the longest on average: the
+      // prefix's shares run beside them, and fewer parts are cheaper to join
+      const int64_t beside = batch * nkv * seq.blocks * own_keys / (64 * 2 * 2 * kCus);
+      const int64_t least = std::max<int64_t>(kPrefixSteps, beside * 64 / step_keys(pre, hd, mod));
+      const int64_t k = std::max<int64_t>(1, std::min<int64_t>(kFusedPre / blocks, steps / least));
       const int64_t per = (steps + k - 1) / k, parts = (steps + per - 1) / per;
       p.units = blocks * per * parts;
       p.pp = PagedPrefix{(uint32_t)p.units, (uint32_t)per, (uint32_t)(per * parts), (uint32_t)pre.blocks,
@@ -1064,10 +1081,11 @@ Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int6
     }
     p.pre_wgs = (p.units + p.pp.per - 1) / p.pp.per;
   }
-  const int64_t steps = pre_steps + (max_len - prefix_len + max_rows - 1) / step + 1;
+  const int64_t steps = pre_steps + (own_keys - 1) / step + 1;
   const int64_t wgs = batch * nkv * seq.blocks;
-  const int64_t least = std::max<int64_t>(kMinSplit, kSplitRows * std::min<int64_t>(32 * seq.tiles, max_rows * G));
-  const int64_t ns = std::max<int64_t>(1, std::min<int64_t>(kSeqWgs / wgs, steps * step / least));
+  const int64_t blk_rows = std::min<int64_t>(32 * seq.tiles, (int64_t)max_rows * G);
+  const int64_t ns = std::max<int64_t>(
+      1, std::min<int64_t>((blk_rows > 64 ? kSeqWgs : kSlimWgs) / wgs, steps * step / std::max<int64_t>(kMinSplit, kSplitRows * blk_rows)));
   const int64_t split_steps = (steps + ns - 1) / ns, nsplit = (steps + split_steps - 1) / split_steps;
   p.items = wgs * nsplit;
   const bool direct = fold || (p.wide && p.pt.pre_parts <= 3);
@@ -1101,12 +1119,14 @@ int launch_all(const Plan& p, const PagedAttn& a, hipStream_t st) {
 
 int64_t pe_internal_paged_mfma_bytes(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int64_t max_len,
                                      int64_t prefix_len) {
-  const Plan p = make_plan(M, batch, nh, nkv, hd, max_rows, max_len, prefix_len);
-  return p.o_bytes + p.ml_bytes;
+  const Plan p = make_plan(M, batch, nh, nkv, hd, max_rows, max_len, prefix_len, false);
+  const Plan m = make_plan(M, batch, nh, nkv, hd, max_rows, max_len, prefix_len, true);
+  return std::max(p.o_bytes + p.ml_bytes, m.o_bytes + m.ml_bytes);
 }
 
 int pe_internal_paged_mfma(const PagedAttn& a, int dtype, void* workspace, int64_t workspace_bytes, hipStream_t st) {
-  Plan p = make_plan(a.M, a.batch, a.nh, a.nkv, a.hd, a.max_rows, a.max_len, a.prefix_len);
+  const bool mod = a.softcap > 0.f || a.slopes || a.window > 0;
+  Plan p = make_plan(a.M, a.batch, a.nh, a.nkv, a.hd, a.max_rows, a.max_len, a.prefix_len, mod);
   if (p.o_bytes > 0 && (!workspace || workspace_bytes < p.o_bytes + p.ml_bytes)) return PE_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 15) return PE_ERR_ARG;
   // rows and work units are counted in 32 bits
@@ -1115,7 +1135,6 @@ int pe_internal_paged_mfma(const PagedAttn& a, int dtype, void* workspace, int64
     return PE_ERR_ARG;
   p.pt.o = (float*)workspace;
   p.pt.ml = (float*)((char*)workspace + p.o_bytes);
-  const bool mod = a.softcap > 0.f || a.slopes || a.window > 0;
 #define PE_GO(DT, HD) return mod ? launch_all<DT, HD, true>(p, a, st) : launch_all<DT, HD, false>(p, a, st)
   if (dtype == PE_DTYPE_BF16) {
     if (a.hd == 128) PE_GO(PE_DTYPE_BF16, 128);
