@@ -262,10 +262,12 @@ __global__ __launch_bounds__(256) void kv_write_kernel(
 // Sequence b's private rows p + path[i] move to p + i, i < len, in every layer
 // and KV head of K and V. path[i] >= i, so a run of rows read whole before the
 // first of them is written never reads what an earlier run wrote: a wave moves
-// one (layer, head) of K or V, its lanes split over rows and vectors
-// (kCompactLoads loads, of four 256-byte rows each). Bound by latency: length,
-// path and table entries, then the rows.
-constexpr int kCompactLoads = 4;
+// one run of rows (four of 256 bytes) of kCompactHeads (layer, head) pairs at a
+// time, all loads before the first store. Where the rows lie is worked out once
+// per run, for all those heads: with one pair to a wave those 64-bit products
+// were the kernel's time (18 us for 32 trees of 64 nodes, 8 layers of 32 heads;
+// 33 MB). What is left is the chain length and path, table entries, rows.
+constexpr int kCompactHeads = 8;
 
 template <typename V>
 __global__ __launch_bounds__(256) void kv_compact_paged_kernel(
@@ -286,54 +288,56 @@ __global__ __launch_bounds__(256) void kv_compact_paged_kernel(
     if (first) atomicOr(status, len > max_rows ? PE_ERR_INDEX : PE_ERR_CAPACITY);
     return;
   }
-  const int lh = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (lh >= LH) return;
+  const int lh0 = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kCompactHeads;
+  if (lh0 >= LH) return;
   const int lane = threadIdx.x & 63;
-  const int layer = lh / nkv, h = lh - layer * nkv;
-  uint8_t* pool = (blockIdx.y == 0 ? kp : vp) + layer * layer_bytes;
+  uint8_t* pool = blockIdx.y == 0 ? kp : vp;
   const int32_t* tab = table + b * ld_table;
-  const int mask = (1 << ps_log2) - 1;
-  // byte offset of private row j of this head, -1 where no such row exists
+  const int64_t row_bytes = vpr * (int64_t)sizeof(V), head_bytes = row_bytes << ps_log2;
+  // byte offset of private row j in KV head 0 of layer 0, -1 where no such row exists
   auto row_at = [&](int64_t j) -> int64_t {
     if (j >= (cols << ps_log2)) return -1;
     const int page = tab[j >> ps_log2];
     if (page < 0 || page >= num_pages) return -1;
-    return ((((int64_t)page * nkv + h) << ps_log2) + (j & mask)) * vpr * (int64_t)sizeof(V);
+    return (int64_t)page * nkv * head_bytes + (j & ((1 << ps_log2) - 1)) * row_bytes;
   };
   const int lanes = min(64, vpr);  // lanes on one row
   const int per = 64 / lanes;      // rows a load instruction moves
   const int sub = lane / lanes, c0 = lane - sub * lanes;
   bool bad = false;
-  for (int base = 0; base < len; base += kCompactLoads * per) {
-    for (int cc = 0; cc < vpr; cc += lanes) {
-      const int c = cc + c0;
-      V v[kCompactLoads];
-      int64_t to[kCompactLoads];
-#pragma unroll
-      for (int k = 0; k < kCompactLoads; ++k) {
-        to[k] = -1;
-        const int i = base + k * per + sub;
-        if (sub < per && i < len && c < vpr) {
-          const int n = res[2 + i];
-          if (n < i || n >= max_rows) {
-            bad = true;
-          } else if (n != i) {
-            const int64_t from = row_at(p + n), dst = row_at(p + i);
-            if (from < 0 || dst < 0) {
-              bad = true;
-            } else {
-              to[k] = dst;
-              v[k] = *(const V*)(pool + from + c * (int64_t)sizeof(V));
-            }
-          }
+  for (int base = 0; base < len; base += per) {
+    const int i = base + sub;
+    int64_t from = -1, dst = -1;
+    if (sub < per && i < len) {
+      const int n = res[2 + i];
+      if (n < i || n >= max_rows) {
+        bad = true;
+      } else if (n != i) {
+        from = row_at(p + n);
+        dst = row_at(p + i);
+        if (from < 0 || dst < 0) {
+          bad = true;
+          dst = -1;
         }
       }
+    }
+    for (int c = c0; c < vpr; c += lanes) {
+      V v[kCompactHeads];
 #pragma unroll
-      for (int k = 0; k < kCompactLoads; ++k)
-        if (to[k] >= 0) *(V*)(pool + to[k] + c * (int64_t)sizeof(V)) = v[k];
+      for (int k = 0; k < kCompactHeads; ++k) {
+        const int layer = (lh0 + k) / nkv, h = lh0 + k - layer * nkv;
+        if (lh0 + k < LH && dst >= 0)
+          v[k] = *(const V*)(pool + layer * layer_bytes + h * head_bytes + from + c * (int64_t)sizeof(V));
+      }
+#pragma unroll
+      for (int k = 0; k < kCompactHeads; ++k) {
+        const int layer = (lh0 + k) / nkv, h = lh0 + k - layer * nkv;
+        if (lh0 + k < LH && dst >= 0)
+          *(V*)(pool + layer * layer_bytes + h * head_bytes + dst + c * (int64_t)sizeof(V)) = v[k];
+      }
     }
   }
-  if (bad && lh == 0 && blockIdx.y == 0) atomicOr(status, PE_ERR_INDEX);
+  if (bad && lh0 == 0 && blockIdx.y == 0) atomicOr(status, PE_ERR_INDEX);
 }
 
 // ---------------------------------------------------------------------------
@@ -593,7 +597,7 @@ extern "C" int pe_kv_compact_paged(void* k_pool, void* v_pool, int L, int nkv, i
   const int64_t row = (int64_t)hd * es;
   const uint64_t any = (uint64_t)(uintptr_t)k_pool | (uint64_t)(uintptr_t)v_pool | (uint64_t)row;
   const int64_t layer_bytes = num_pages * nkv * page_size * row;
-  const dim3 grid(pe_cdiv((int64_t)L * nkv, 4), 2, batch);
+  const dim3 grid(pe_cdiv((int64_t)L * nkv, 4 * kCompactHeads), 2, batch);
   hipStream_t st = (hipStream_t)stream;
 #define PE_COMPACT(V)                                                                                             \
   kv_compact_paged_kernel<V><<<grid, 256, 0, st>>>((uint8_t*)k_pool, (uint8_t*)v_pool, layer_bytes, L * nkv, nkv, \
