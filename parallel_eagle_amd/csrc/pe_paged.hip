@@ -230,30 +230,33 @@ __global__ __launch_bounds__(256) void kv_write_kernel(
   const uint8_t* src = (is_v ? vs : ks) + layer * (is_v ? sl_v : sl_k);
   const int64_t sr = is_v ? sr_v : sr_k, sh = is_v ? sh_v : sh_k;
   uint8_t* dst = (is_v ? vp : kp) + layer * layer_bytes;
-  const int64_t total = (int64_t)M * nkv * vpr;  // vectors
-  const int64_t first = (int64_t)blockIdx.x * 256 * kWriteUnroll + threadIdx.x;
+  const uint32_t total = (uint32_t)M * (uint32_t)nkv * (uint32_t)vpr;  // vectors (below 2^31)
+  const uint32_t start = blockIdx.x * (256 * kWriteUnroll) + threadIdx.x;
   V v[kWriteUnroll];
-  int64_t to[kWriteUnroll];
+  int64_t slot[kWriteUnroll];
+  uint32_t head[kWriteUnroll], col[kWriteUnroll];
 #pragma unroll
-  for (int u = 0; u < kWriteUnroll; ++u) {
-    const int64_t i = first + u * 256;
-    to[u] = -1;
+  for (int u = 0; u < kWriteUnroll; ++u) {  // a row's slot and its values are asked for together
+    const uint32_t i = start + u * 256;
+    slot[u] = -1;
     if (i < total) {
-      const uint32_t piece = (uint32_t)(i / vpr), c = (uint32_t)(i - (int64_t)piece * vpr);
-      const uint32_t h = piece / (uint32_t)M, r = piece - h * (uint32_t)M;
-      const int64_t slot = slots[r];
-      if (slot >= 0 && slot < num_slots) {
-        const int64_t page = slot >> ps_log2, at = slot & ((1 << ps_log2) - 1);
-        to[u] = ((((page * nkv + h) << ps_log2) + at) * vpr + c) * (int64_t)sizeof(V);
-        v[u] = *(const V*)(src + r * sr + h * sh + c * sizeof(V));
-      } else if (slot != -1 && !is_v && layer == 0 && h == 0 && c == 0) {
-        atomicOr(status, PE_ERR_INDEX);
-      }
+      const uint32_t piece = i / (uint32_t)vpr;
+      col[u] = i - piece * vpr;
+      head[u] = piece / (uint32_t)M;
+      const uint32_t r = piece - head[u] * M;
+      slot[u] = slots[r];
+      v[u] = *(const V*)(src + r * sr + head[u] * sh + col[u] * sizeof(V));
     }
   }
 #pragma unroll
-  for (int u = 0; u < kWriteUnroll; ++u)
-    if (to[u] >= 0) *(V*)(dst + to[u]) = v[u];
+  for (int u = 0; u < kWriteUnroll; ++u) {
+    if (slot[u] >= 0 && slot[u] < num_slots) {
+      const int64_t page = slot[u] >> ps_log2, at = slot[u] & ((1 << ps_log2) - 1);
+      *(V*)(dst + ((((page * nkv + head[u]) << ps_log2) + at) * vpr + col[u]) * (int64_t)sizeof(V)) = v[u];
+    } else if (slot[u] != -1 && !is_v && layer == 0 && head[u] == 0 && col[u] == 0) {
+      atomicOr(status, PE_ERR_INDEX);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -570,7 +573,7 @@ extern "C" int pe_kv_write_paged(const void* k, const void* v, const int64_t* k_
   do {                                                                                                            \
     const int vpr = (int)(row / (int64_t)sizeof(V));                                                              \
     const int64_t blocks = (M * nkv * vpr + 256 * kWriteUnroll - 1) / (256 * kWriteUnroll);                       \
-    if (blocks >= (int64_t(1) << 31)) return PE_ERR_ARG;                                                          \
+    if (M * nkv * vpr >= (int64_t(1) << 31)) return PE_ERR_ARG;                                                   \
     kv_write_kernel<V><<<dim3((unsigned)blocks, L, 2), 256, 0, st>>>(                                             \
         (const uint8_t*)k, (const uint8_t*)v, k_strides[0] * es, k_strides[1] * es, k_strides[2] * es,            \
         v_strides[0] * es, v_strides[1] * es, v_strides[2] * es, (uint8_t*)k_pool, (uint8_t*)v_pool, layer_bytes, \
