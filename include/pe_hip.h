@@ -555,6 +555,21 @@ typedef struct pe_pass_args {
    * [M][pe_dense_gemm_argmax_groups(M, vocab, hidden)] (see
    * pe_dense_gemm_argmax), for pe_accept_tree_keys. NULL: none. */
   uint64_t* node_keys;
+  /* Paged batch (page_size > 0, batch >= 1; 0 = the contiguous caches above):
+   * k_cache / v_cache are pools [L][num_pages][nkv][page_size][hd] (see the
+   * paged cache), row r's K/V go to slots[r] (device int64 [M], from
+   * pe_page_tables; -1 drops them), and attention runs over the shared_len
+   * tokens of prefix_table, each sequence's pages and its rows. seq_prefix[b]
+   * counts all cached tokens of sequence b, the shared ones included, and
+   * prefix_len bounds it. PE_MASK_TREE, or PE_MASK_CAUSAL for rows that are
+   * consecutive tokens (chunks of prompts; positions as given). The same models
+   * as the contiguous batch; cache_capacity and cache_seq_stride are not read. */
+  const int64_t* slots;
+  const int32_t* block_table; /* [batch][table_cols], rows ld_table apart */
+  const int32_t* prefix_table; /* [prefix_pages], NULL when shared_len is 0 */
+  int64_t ld_table, table_cols, num_pages, prefix_pages, shared_len;
+  int32_t page_size;
+  int32_t _pad2;
 } pe_pass_args;
 
 /* Workspace for pe_forward with up to M rows and kv_len = P + M keys. */
@@ -563,6 +578,10 @@ int64_t pe_forward_workspace_bytes(const pe_model_desc* m, int M, int64_t kv_len
  * sequence, at most max_kv_len = prefix + rows keys per sequence. */
 int64_t pe_forward_batch_workspace_bytes(const pe_model_desc* m, int M, int max_seq_rows, int64_t max_kv_len,
                                          int batch);
+/* Workspace for a paged pe_forward of the same sizes: max_len bounds the cached
+ * tokens of a sequence (shared ones included). */
+int64_t pe_forward_paged_workspace_bytes(const pe_model_desc* m, int M, int max_seq_rows, int64_t max_len, int batch,
+                                         int64_t shared_len);
 /* The masked verification forward TargetModel.forward_cached
  * (src/pe/target.py:203-224 -> HF LlamaForCausalLM / Qwen2ForCausalLM forward,
  * modeling_llama.py:347-490): embeddings, L decoder layers with in-place KV

@@ -88,7 +88,9 @@ class PassArgs(C.Structure):
         ("_pad", i32), ("k_cache", vp), ("v_cache", vp), ("cache_capacity", i64), ("logits", vp),
         ("fused", vp), ("workspace", vp), ("workspace_bytes", i64), ("status", vp),
         ("batch", i32), ("max_seq_rows", i32), ("seq_row0", vp), ("seq_prefix", vp), ("cache_seq_stride", i64),
-        ("node_keys", vp),
+        ("node_keys", vp), ("slots", vp), ("block_table", vp), ("prefix_table", vp), ("ld_table", i64),
+        ("table_cols", i64), ("num_pages", i64), ("prefix_pages", i64), ("shared_len", i64), ("page_size", i32),
+        ("_pad2", i32),
     ]
 
 
@@ -157,6 +159,7 @@ SIGNATURES: dict[str, tuple] = {
     "pe_forward_workspace_bytes": (i64, [C.POINTER(ModelDesc), C.c_int, i64]),
     "pe_forward": (C.c_int, [C.POINTER(ModelDesc), C.POINTER(PassArgs), vp]),
     "pe_forward_batch_workspace_bytes": (i64, [C.POINTER(ModelDesc), C.c_int, C.c_int, i64, C.c_int]),
+    "pe_forward_paged_workspace_bytes": (i64, [C.POINTER(ModelDesc), C.c_int, C.c_int, i64, C.c_int, i64]),
     "pe_tree_masks_batch": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, vp, C.c_int, vp, vp, vp, vp]),
     "pe_accept_tree_batch": (C.c_int, [vp, i64, vp, i64, i64, C.c_int, vp, C.c_int, C.c_int, vp, vp, vp, vp, vp]),
     "pe_kv_compact_batch": (C.c_int, [vp, vp, C.c_int, i64, C.c_int, C.c_int, i64, C.c_int, C.c_int, vp, vp,

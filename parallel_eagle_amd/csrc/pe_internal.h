@@ -161,3 +161,9 @@ PE_INTERNAL int pe_internal_kv_offsets(const int32_t* seq_row0, const int64_t* s
                                        int64_t seq_stride, int64_t cap, int hd, int64_t max_prefix, int max_rows,
                                        int64_t* off, int32_t* status, hipStream_t st);
 
+// pe_paged.hip: pe_tree_attention_paged whose output is A-tiled when out_units >
+// 0 (16-bit, hd 64 or 128, aligned as its matrix-core kernels need).
+PE_INTERNAL int pe_internal_tree_attention_paged(const pe_paged_attention_args* p, int out_units, hipStream_t st);
+// pe_paged.hip: per-row K/V offsets of a paged pass (EpiArgs::kv_off) from its slots.
+PE_INTERNAL int pe_internal_slot_offsets(const int64_t* slots, int M, int nkv, int hd, int page_size, int64_t num_pages,
+                                         int64_t* off, int32_t* status, hipStream_t st);

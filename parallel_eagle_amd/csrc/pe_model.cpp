@@ -514,8 +514,10 @@ bool batch_big_path(const pe_model_desc* m, int M) {
          nqkv % 128 == 0;
 }
 
+// `shared` >= 0: a paged pass behind that many shared tokens (max_kv_len its
+// longest sequence and rows).
 BatchLayout make_batch_layout(const pe_model_desc* m, int M, int max_rows, int64_t max_kv_len, int batch,
-                              bool many = true) {
+                              bool many = true, int64_t shared = -1) {
   BatchLayout L;
   const int es = esize(m->dtype);
   const int H = m->hidden, qd = m->num_heads * m->head_dim, ip = m->intermediate_padded;
@@ -541,8 +543,10 @@ BatchLayout make_batch_layout(const pe_model_desc* m, int M, int max_rows, int64
   L.attn = take((int64_t)M * qd * es);
   L.act = take((int64_t)M * ip * es);
   L.kvoff = take((int64_t)M * 8);
-  L.attn_ws_bytes =
-      align_up(pe_internal_attention_batch_bytes(max_rows, m->num_heads, m->num_kv_heads, max_kv_len, batch));
+  L.attn_ws_bytes = align_up(
+      shared < 0 ? pe_internal_attention_batch_bytes(max_rows, m->num_heads, m->num_kv_heads, max_kv_len, batch)
+                 : pe_attention_paged_workspace_bytes(M, batch, m->num_heads, m->num_kv_heads, m->head_dim, max_rows,
+                                                      max_kv_len - max_rows, shared, m->dtype));
   L.attn_ws = take(L.attn_ws_bytes);
   L.big = many && batch_big_path(m, M);
   L.xn_t = L.attn_t = L.act_t = L.part = L.part_bytes = 0;
@@ -589,7 +593,10 @@ int forward_batched(const pe_model_desc* m, const pe_pass_args* a, const BatchLa
   char* act = ws + Lb.act;
   int64_t* kvoff = (int64_t*)(ws + Lb.kvoff);
   const float scale = (float)(1.0 / std::sqrt((double)hd));
-  const int64_t layer_stride = (int64_t)nkv * a->cache_capacity * hd * es;
+  // a page takes a cache's place: the epilogues' rows of a head are page_size apart
+  const bool paged = a->page_size > 0;
+  const int64_t cap = paged ? a->page_size : a->cache_capacity;
+  const int64_t layer_stride = (int64_t)nkv * cap * hd * es * (paged ? a->num_pages : 1);
   const int64_t fused_ld = (int64_t)a->num_features * H;
   int rc;
 #define PE_TRY(expr)            \
@@ -597,6 +604,45 @@ int forward_batched(const pe_model_desc* m, const pe_pass_args* a, const BatchLa
     rc = (expr);                \
     if (rc != PE_OK) return rc; \
   } while (0)
+  auto attention = [&](const void* kc, const void* vc, void* out, int units) -> int {
+    if (!paged)
+      return pe_internal_tree_attention_batch(q, kc, vc, a->cache_capacity, a->cache_seq_stride, nh, nkv,
+                                              a->max_seq_rows, a->prefix_len, a->batch, a->seq_row0, a->seq_prefix,
+                                              a->tree_bits, a->bits_words, scale, m->dtype, out, qd, units,
+                                              ws + Lb.attn_ws, Lb.attn_ws_bytes, (int*)gws + kPassAttnCounterInt, st);
+    pe_paged_attention_args p = {};
+    p.q = q;
+    p.k_pool = kc;
+    p.v_pool = vc;
+    p.out = out;
+    p.block_table = a->block_table;
+    p.prefix_table = a->prefix_table;
+    p.seq_row0 = a->seq_row0;
+    p.seq_len = a->seq_prefix;
+    p.bits = a->tree_bits;
+    p.workspace = ws + Lb.attn_ws;
+    p.status = a->status;
+    p.workspace_bytes = Lb.attn_ws_bytes;
+    p.ld_q = p.ld_out = qd;
+    p.ld_table = a->ld_table;
+    p.table_cols = a->table_cols;
+    p.num_pages = a->num_pages;
+    p.prefix_pages = a->prefix_pages;
+    p.prefix_len = a->shared_len;
+    p.max_len = a->prefix_len;
+    p.M = M;
+    p.batch = a->batch;
+    p.max_rows = a->max_seq_rows;
+    p.nh = nh;
+    p.nkv = nkv;
+    p.hd = hd;
+    p.page_size = a->page_size;
+    p.dtype = m->dtype;
+    p.mask_mode = a->mask_mode;
+    p.words = a->bits_words;
+    p.scale = scale;
+    return pe_internal_tree_attention_paged(&p, units, st);
+  };
   auto slot_of = [&](int layer) -> int {
     if (!a->fused) return -1;
     for (int f = 0; f < a->num_features; ++f)
@@ -613,8 +659,11 @@ int forward_batched(const pe_model_desc* m, const pe_pass_args* a, const BatchLa
     }
     return PE_OK;
   };
-  PE_TRY(pe_internal_kv_offsets(a->seq_row0, a->seq_prefix, a->batch, M, a->cache_seq_stride, a->cache_capacity, hd,
-                                a->prefix_len, a->max_seq_rows, kvoff, a->status, st));
+  if (paged)
+    PE_TRY(pe_internal_slot_offsets(a->slots, M, nkv, hd, a->page_size, a->num_pages, kvoff, a->status, st));
+  else
+    PE_TRY(pe_internal_kv_offsets(a->seq_row0, a->seq_prefix, a->batch, M, a->cache_seq_stride, a->cache_capacity, hd,
+                                  a->prefix_len, a->max_seq_rows, kvoff, a->status, st));
   char* xn_t = Lb.big ? ws + Lb.xn_t : nullptr;
   {
     const int f0 = slot_of(0);
@@ -639,12 +688,9 @@ int forward_batched(const pe_model_desc* m, const pe_pass_args* a, const BatchLa
       PE_TRY(pe_internal_many_linear(wf, m->dtype, xn_t, M, H, m->w_qkv[l], m->a_qkv ? m->a_qkv[l] : nullptr, nqkv, part,
                                      Lb.part_bytes, &S, st));
       PE_TRY(pe_internal_rope_kv_partials(part, S, M, nh, nkv, hd, m->b_qkv ? m->b_qkv[l] : nullptr, a->positions,
-                                          m->rope_cos_sin, m->max_positions, q, kc, vc, a->cache_capacity, 0,
+                                          m->rope_cos_sin, m->max_positions, q, kc, vc, cap, 0,
                                           a->status, m->dtype, st, kvoff));
-      PE_TRY(pe_internal_tree_attention_batch(q, kc, vc, a->cache_capacity, a->cache_seq_stride, nh, nkv,
-                                              a->max_seq_rows, a->prefix_len, a->batch, a->seq_row0, a->seq_prefix,
-                                              a->tree_bits, a->bits_words, scale, m->dtype, attn_t, qd, qd / 128,
-                                              ws + Lb.attn_ws, Lb.attn_ws_bytes, (int*)gws + kPassAttnCounterInt, st));
+      PE_TRY(attention(kc, vc, attn_t, qd / 128));
       PE_TRY(pe_internal_many_linear(wf, m->dtype, attn_t, M, qd, m->w_o[l], m->a_o ? m->a_o[l] : nullptr, H, part,
                                      Lb.part_bytes, &S, st));
       PE_TRY(pe_internal_residual_rmsnorm(part, S, M, h, H, m->mlp_norm[l], m->rms_eps, m->norm_mode, m->dtype, xn,
@@ -680,13 +726,10 @@ int forward_batched(const pe_model_desc* m, const pe_pass_args* a, const BatchLa
       const int mc = M - c0 < kFusedChunk ? M - c0 : kFusedChunk;
       PE_TRY(pe_internal_gemm_rope_kv(wf, m->dtype, xn + (int64_t)c0 * H * es, H, mc, H, m->w_qkv[l], a_qkv, nh, nkv,
                                       hd, b_qkv, a->positions + c0, m->rope_cos_sin, m->max_positions,
-                                      q + (int64_t)c0 * qd * es, kc, vc, a->cache_capacity, 0, a->status, gws, gwsb,
+                                      q + (int64_t)c0 * qd * es, kc, vc, cap, 0, a->status, gws, gwsb,
                                       false, st, kvoff + c0));
     }
-    PE_TRY(pe_internal_tree_attention_batch(q, kc, vc, a->cache_capacity, a->cache_seq_stride, nh, nkv,
-                                            a->max_seq_rows, a->prefix_len, a->batch, a->seq_row0, a->seq_prefix,
-                                            a->tree_bits, a->bits_words, scale, m->dtype, attn, qd, 0, ws + Lb.attn_ws,
-                                            Lb.attn_ws_bytes, (int*)gws + kPassAttnCounterInt, st));
+    PE_TRY(attention(kc, vc, attn, 0));
     const void* a_o = m->a_o ? m->a_o[l] : nullptr;
     PE_TRY(pe_internal_linear(wf, m->dtype, attn, qd, false, M, qd, m->w_o[l], a_o, H, PE_EPI_RESIDUAL, nullptr, h, H,
                               h, H, 0, gws, gwsb, st));
@@ -725,6 +768,28 @@ extern "C" int64_t pe_forward_batch_workspace_bytes(const pe_model_desc* m, int 
   return b;
 }
 
+extern "C" int64_t pe_forward_paged_workspace_bytes(const pe_model_desc* m, int M, int max_seq_rows, int64_t max_len,
+                                                    int batch, int64_t shared_len) {
+  if (!m || M <= 0 || max_seq_rows <= 0 || shared_len < 0 || max_len < shared_len || batch <= 0) return 0;
+  return make_batch_layout(m, M, max_seq_rows, max_len + max_seq_rows, batch, true, shared_len).total;
+}
+
+// A batched pass over paged caches: checks, then the batched pass.
+static int forward_paged(const pe_model_desc* m, const pe_pass_args* a, hipStream_t st) {
+  const int M = a->M;
+  if (a->batch <= 0 || !a->seq_row0 || !a->seq_prefix || !a->slots || !a->block_table || !a->status || a->node_keys ||
+      a->num_pages <= 0 || a->shared_len < 0 || a->prefix_len < a->shared_len)
+    return PE_ERR_ARG;
+  if (m->dtype == PE_DTYPE_F32 || m->head_dim != 128 || m->qkv_layout != PE_QKV_ROPE_PAIRED ||
+      m->attn_mode != PE_ATTN_SDPA)
+    return PE_ERR_ARG;
+  if (a->max_seq_rows <= 0 || a->max_seq_rows > M) return PE_ERR_TREE;
+  const BatchLayout Lb = make_batch_layout(m, M, a->max_seq_rows, a->prefix_len + a->max_seq_rows, a->batch, true,
+                                           a->shared_len);
+  if (a->workspace_bytes < Lb.total) return PE_ERR_WORKSPACE;
+  return forward_batched(m, a, Lb, st);
+}
+
 extern "C" int pe_forward(const pe_model_desc* m, const pe_pass_args* a, void* stream) {
   if (!m || !a) return PE_ERR_ARG;
   const int M = a->M;
@@ -732,7 +797,7 @@ extern "C" int pe_forward(const pe_model_desc* m, const pe_pass_args* a, void* s
   // a batched pass appends at most max_seq_rows rows to any one cache (each
   // row's slot is checked again on the device against its own prefix)
   const int64_t appended = a->batch > 0 ? a->max_seq_rows : M;
-  if (a->prefix_len < 0 || a->prefix_len + appended > a->cache_capacity) return PE_ERR_CAPACITY;
+  if (a->prefix_len < 0 || (a->page_size == 0 && a->prefix_len + appended > a->cache_capacity)) return PE_ERR_CAPACITY;
   if (a->num_features < 0 || a->num_features > 4) return PE_ERR_ARG;
   if (a->mask_mode == PE_MASK_TREE && !a->tree_bits) return PE_ERR_ARG;
   if (m->intermediate_padded % 32 || m->intermediate_padded < m->intermediate) return PE_ERR_ARG;
@@ -742,7 +807,8 @@ extern "C" int pe_forward(const pe_model_desc* m, const pe_pass_args* a, void* s
   // models with eager attention run the fused pass on row-major activations)
   if (m->attn_mode == PE_ATTN_EAGER && pe_wfmt_nf4(m->weight_format)) return PE_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;
-  if (a->batch < 0) return PE_ERR_ARG;
+  if (a->batch < 0 || a->page_size < 0) return PE_ERR_ARG;
+  if (a->page_size > 0) return forward_paged(m, a, st);
   // argmax keys: single-sequence 16-bit passes of at most one chunk that write
   // logits (a batch of one included)
   if (a->node_keys && (a->batch > 1 || !a->logits || m->dtype == PE_DTYPE_F32 || M > kFusedChunk))

@@ -21,6 +21,7 @@ struct PagedAttn {
   int64_t ld_q, ld_out, ld_table, cols, num_pages, prefix_len, max_len, window, M;
   int batch, max_rows, nh, nkv, hd, ps_log2, mask_mode, words;
   float scale, softcap;
+  int out_units;  // > 0: out is A-tiled over all rows (nh * hd = 128 * out_units; matrix-core kernels only)
 };
 
 // the running maximum of a row that has seen nothing (its sum is 0)
@@ -50,6 +51,13 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttn& a, int b) {
     s.err = PE_ERR_CAPACITY;
   s.ok = s.err == 0 && s.rows > 0;
   return s;
+}
+
+// Four consecutive columns of a token's output row.
+template <int DT>
+__device__ __forceinline__ void paged_out4(const PagedAttn& a, int64_t tok, int col, const float (&v)[4]) {
+  typedef typename Elem<DT>::T Te;
+  Vec4<DT>::store((Te*)a.out + (a.out_units ? xtile_index((int)tok, col, a.out_units) : tok * a.ld_out + col), v);
 }
 
 // pe_paged.hip: the call on the VALU (fp32, any head size up to 256).

@@ -259,6 +259,20 @@ __global__ __launch_bounds__(256) void kv_write_kernel(
   }
 }
 
+// Element offset of each row's slot in head 0 of a layer's pool, -1 for a row
+// without one: what the q/k/v epilogues of a pass take (head h adds h *
+// page_size * hd there).
+__global__ __launch_bounds__(256) void slot_offsets_kernel(const int64_t* __restrict__ slots, int M, int nkv, int hd,
+                                                           int ps_log2, int64_t num_slots, int64_t* __restrict__ off,
+                                                           int32_t* status) {
+  const int r = blockIdx.x * 256 + threadIdx.x;
+  if (r >= M) return;
+  const int64_t s = slots[r];
+  const bool ok = s >= 0 && s < num_slots;
+  if (!ok && s != -1 && status) atomicOr(status, PE_ERR_INDEX);
+  off[r] = ok ? ((((s >> ps_log2) * nkv) << ps_log2) + (s & ((1 << ps_log2) - 1))) * hd : -1;
+}
+
 // ---------------------------------------------------------------------------
 // Accepted rows together
 // ---------------------------------------------------------------------------
@@ -511,6 +525,15 @@ int pe_internal_paged_valu(const PagedAttn& a, int dtype, hipStream_t st) {
   return PE_OK;
 }
 
+int pe_internal_slot_offsets(const int64_t* slots, int M, int nkv, int hd, int page_size, int64_t num_pages,
+                             int64_t* off, int32_t* status, hipStream_t st) {
+  const int psl = page_log2(page_size);
+  if (!slots || !off || M <= 0 || psl < 0 || num_pages <= 0) return PE_ERR_ARG;
+  slot_offsets_kernel<<<pe_cdiv(M, 256), 256, 0, st>>>(slots, M, nkv, hd, psl, num_pages * page_size, off, status);
+  PE_CHECK_LAUNCH();
+  return PE_OK;
+}
+
 extern "C" int64_t pe_page_tables_scratch_bytes(int batch) { return batch < 0 ? 0 : 4 * ((int64_t)batch + 1); }
 
 extern "C" int pe_page_tables(const int64_t* seq_len, const int32_t* seq_row0, int batch, int64_t M,
@@ -629,6 +652,10 @@ extern "C" int64_t pe_attention_paged_workspace_bytes(int64_t M, int batch, int 
 }
 
 extern "C" int pe_tree_attention_paged(const pe_paged_attention_args* p, void* stream) {
+  return pe_internal_tree_attention_paged(p, 0, (hipStream_t)stream);
+}
+
+int pe_internal_tree_attention_paged(const pe_paged_attention_args* p, int out_units, hipStream_t st) {
   if (!p) return PE_ERR_ARG;
   const int es = esize(p->dtype), psl = page_log2(p->page_size);
   const bool none = p->M == 0 || p->max_rows == 0;  // no rows: their buffers may be absent
@@ -685,7 +712,9 @@ extern "C" int pe_tree_attention_paged(const pe_paged_attention_args* p, void* s
   a.softcap = p->softcap;
   const bool aligned = (((uintptr_t)p->q | (uintptr_t)p->k_pool | (uintptr_t)p->v_pool | (uintptr_t)p->out) & 15) == 0 &&
                        p->ld_q % 8 == 0 && p->ld_out % 8 == 0;
+  a.out_units = out_units;
   if (mfma_fits(p->hd, p->dtype) && aligned)
-    return pe_internal_paged_mfma(a, p->dtype, p->workspace, p->workspace_bytes, (hipStream_t)stream);
-  return pe_internal_paged_valu(a, p->dtype, (hipStream_t)stream);
+    return pe_internal_paged_mfma(a, p->dtype, p->workspace, p->workspace_bytes, st);
+  if (out_units) return PE_ERR_ARG;
+  return pe_internal_paged_valu(a, p->dtype, st);
 }

@@ -797,17 +797,15 @@ __device__ __forceinline__ int splits_of(const PagedSeqs& sq, const PagedSeq& s)
 }
 
 template <int DT, int OB>
-__device__ __forceinline__ void write_out(const PagedAttn& a, int64_t tok, int64_t col, const f32x16_t (&o)[OB],
+__device__ __forceinline__ void write_out(const PagedAttn& a, int64_t tok, int col, const f32x16_t (&o)[OB],
                                           float l) {
-  typedef typename Elem<DT>::T Te;
-  Te* dst = (Te*)a.out + tok * a.ld_out + col;
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int h = 0; h < OB; ++h)
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const float v[4] = {o[h][4 * c] * inv, o[h][4 * c + 1] * inv, o[h][4 * c + 2] * inv, o[h][4 * c + 3] * inv};
-      Vec4<DT>::store(dst + 32 * h + 8 * c, v);
+      paged_out4<DT>(a, tok, col + 32 * h + 8 * c, v);
     }
 }
 
@@ -910,7 +908,7 @@ __device__ __forceinline__ void seq_item(const PagedAttn& a, const PagedPrefix& 
         }
     }
   }
-  write_out<DT, C::OB>(a, tok, (int64_t)hq * HD + 32 * hb + 4 * g, o, l);
+  write_out<DT, C::OB>(a, tok, hq * HD + 32 * hb + 4 * g, o, l);
 }
 
 // ---------------------------------------------------------------------------
@@ -1006,10 +1004,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefi
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-  typedef typename Elem<DT>::T Te;
   const uint32_t tok = grow / G;
   const int hq = (int)(kvh * G + (grow - tok * G));
-  Vec4<DT>::store((Te*)a.out + tok * a.ld_out + (int64_t)hq * HD + 4 * piece, v);
+  paged_out4<DT>(a, tok, hq * HD + 4 * piece, v);
 }
 
 // ------------------------------------------------------------------ plans
