@@ -698,6 +698,14 @@ def register_torch_ops() -> None:
     - ``kv_compact(k_cache!, v_cache!, prefix_len, accept_out)`` and
       ``kv_gather(k_cache!, v_cache!, keep, status!)``: gather_cache
       (src/pe/target.py:194-201);
+    - ``page_tables(seq_len, seq_row0, block_table!, held!, free_pages, free_top!,
+      page_size, rows, prefix_len, status!) -> slots``, ``kv_write_paged(k, v,
+      k_pool!, v_pool!, slots, status!)``, ``kv_compact_paged(k_pool!, v_pool!,
+      block_table, seq_len, accept_out, prefix_len, status!)`` and
+      ``tree_attention_paged(q, k_pool, v_pool, block_table, seq_row0, seq_len,
+      scale, max_rows, max_len, status!, mask_mode, bits?, positions?,
+      prefix_table?, prefix_len, softcap, slopes?, window) -> out``: the paged
+      cache and the attention that reads it;
     - ``rmsnorm``, ``argmax_rows``, ``nf4_linear``, ``dense_linear``: the pass's
       building blocks.
     """
@@ -760,6 +768,50 @@ def register_torch_ops() -> None:
     @_kv_gather.register_fake
     def _(k_cache, v_cache, keep, status):
         return None
+
+    @op("page_tables", "(Tensor seq_len, Tensor seq_row0, Tensor(a!) block_table, Tensor(b!) held, Tensor free_pages, "
+        "Tensor(c!) free_top, int page_size, int rows, int prefix_len, Tensor(d!) status) -> Tensor",
+        ("block_table", "held", "free_top", "status"))
+    def _page_tables(seq_len, seq_row0, block_table, held, free_pages, free_top, page_size, rows, prefix_len, status):
+        return page_tables(seq_len, seq_row0, block_table, held, free_pages, free_top, page_size, rows, status,
+                           prefix_len=prefix_len)
+
+    @_page_tables.register_fake
+    def _(seq_len, seq_row0, block_table, held, free_pages, free_top, page_size, rows, prefix_len, status):
+        return seq_len.new_empty(rows)
+
+    @op("kv_write_paged", "(Tensor k, Tensor v, Tensor(a!) k_pool, Tensor(b!) v_pool, Tensor slots, Tensor(c!) status) "
+        "-> ()", ("k_pool", "v_pool", "status"))
+    def _kv_write_paged(k, v, k_pool, v_pool, slots, status):
+        kv_write_paged(k, v, k_pool, v_pool, slots, status)
+
+    @_kv_write_paged.register_fake
+    def _(k, v, k_pool, v_pool, slots, status):
+        return None
+
+    @op("kv_compact_paged", "(Tensor(a!) k_pool, Tensor(b!) v_pool, Tensor block_table, Tensor seq_len, "
+        "Tensor accept_out, int prefix_len, Tensor(c!) status) -> ()", ("k_pool", "v_pool", "status"))
+    def _kv_compact_paged(k_pool, v_pool, block_table, seq_len, accept_out, prefix_len, status):
+        kv_compact_paged(k_pool, v_pool, block_table, seq_len, accept_out, status, prefix_len=prefix_len)
+
+    @_kv_compact_paged.register_fake
+    def _(k_pool, v_pool, block_table, seq_len, accept_out, prefix_len, status):
+        return None
+
+    @op("tree_attention_paged", "(Tensor q, Tensor k_pool, Tensor v_pool, Tensor block_table, Tensor seq_row0, "
+        "Tensor seq_len, float scale, int max_rows, int max_len, Tensor(a!) status, int mask_mode, Tensor? bits, "
+        "Tensor? positions, Tensor? prefix_table, int prefix_len, float softcap, Tensor? slopes, int window) -> Tensor",
+        ("status",))
+    def _tree_attention_paged(q, k_pool, v_pool, block_table, seq_row0, seq_len, scale, max_rows, max_len, status,
+                              mask_mode, bits, positions, prefix_table, prefix_len, softcap, slopes, window):
+        return tree_attention_paged(q, k_pool, v_pool, block_table, seq_row0, seq_len, scale, max_rows, max_len, status,
+                                    mask_mode=mask_mode, bits=bits, positions=positions, prefix_table=prefix_table,
+                                    prefix_len=prefix_len, softcap=softcap, slopes=slopes, window=window)
+
+    @_tree_attention_paged.register_fake
+    def _(q, k_pool, v_pool, block_table, seq_row0, seq_len, scale, max_rows, max_len, status, mask_mode, bits, positions,
+          prefix_table, prefix_len, softcap, slopes, window):
+        return q.new_empty((q.shape[0], q.shape[1] * q.shape[2]))
 
     @op("rmsnorm", "(Tensor x, Tensor w, float eps) -> Tensor")
     def _rmsnorm(x, w, eps):

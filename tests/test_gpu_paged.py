@@ -578,3 +578,86 @@ def test_compact_flags_paths_and_pages_that_are_none():
     assert call([1, 0, 2, 0, 0], length=31)[0] == _lib.PE_ERR_INDEX  # past the table
     assert call([1, 0, 2, 0, 0], length=-1) == (_lib.PE_ERR_CAPACITY, True)
     assert call([1, 0, 2, 0, 0], length=32) == (_lib.PE_ERR_CAPACITY, True)
+
+
+# ------------------------------------------------------------------ together
+def test_torch_ops_equal_the_wrappers():
+    ops.register_torch_ops()
+    c = Case((10, 2, 128), [26, 9], [40, 100], 70, dtype=torch.float16, seed=20, cap=20.0, window=90, bias=True)
+    want = c.run()
+    got = torch.ops.pe.tree_attention_paged(c.q, c.k_pool, c.v_pool, c.table, c.seq_row0, c.seq_len, c.scale, c.max_rows,
+                                            c.max_len, c.status, TREE, c.bits, c.positions, c.ptab, c.prefix, 20.0,
+                                            c.slopes, 90)
+    assert torch.equal(got, want)
+    t = lambda x, d=torch.int32: torch.tensor(x, dtype=d, device=DEV)
+    table, held, free, top, st = t([[-1, -1]] * 2), t([0, 0]), t(list(range(6))), t([6]), status_word()
+    slots = torch.ops.pe.page_tables(t([0, 0], torch.int64), t([0, 20, 23]), table, held, free, top, 16, 23, 0, st)
+    assert slots.tolist() == [5 * 16 + i for i in range(16)] + [4 * 16 + i for i in range(4)] + [3 * 16 + i for i in range(3)]
+    pools = [torch.zeros((2, 6, 2, 16, 64), dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    rows = torch.randn((2, 23, 2, 64), device=DEV).to(torch.bfloat16)
+    torch.ops.pe.kv_write_paged(rows, rows, pools[0], pools[1], slots, st)
+    acc = torch.zeros((2, 22), dtype=torch.int32, device=DEV)
+    acc[0, 0], acc[0, 2], acc[0, 3] = 2, 3, 17
+    torch.ops.pe.kv_compact_paged(pools[0], pools[1], table, t([0, 0], torch.int64), acc, 0, st)
+    for p in pools:
+        assert torch.equal(p[:, 5, :, 0], rows[:, 3]) and torch.equal(p[:, 5, :, 1], rows[:, 17])
+        assert torch.equal(p[:, 5, :, 2], rows[:, 2]) and torch.equal(p[:, 3, :, 0], rows[:, 20])
+    assert int(st.item()) == 0
+
+
+def test_a_step_of_the_operators_in_one_graph():
+    """Tables, write, attention and commit as a decode step runs them, captured once and replayed as the sequences grow,
+    against the same step on host integers and float64."""
+    nh, nkv, hd, ps, B, T, layers = 8, 2, 128, 16, 3, 5, 2
+    gen = torch.Generator().manual_seed(30)
+    t = lambda x, d=torch.int32: torch.tensor(x, dtype=d, device=DEV)
+    pages = 40
+    pools = [torch.zeros((layers, pages, nkv, ps, hd), dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    table, held, free, top = t([[-1] * 8] * B), t([0] * B), t(list(range(pages))), t([pages])
+    seq_len, row0, st = t([0] * B, torch.int64), t([0, T, 2 * T, 3 * T]), status_word()
+    bits, _ = ancestor_bits([-1, 0, 1, 0, 3], 1)
+    bits = bits.repeat(B, 1).to(DEV)
+    qkv = torch.zeros((layers, B * T, (nh + 2 * nkv) * hd), dtype=torch.bfloat16, device=DEV)
+    acc = t([[3, 0, 0, 3, 4, 0, 0]] * B)  # the path 0, 3, 4
+    out = torch.zeros((B * T, nh * hd), dtype=torch.bfloat16, device=DEV)
+    slots = torch.zeros(B * T, dtype=torch.int64, device=DEV)
+    ws = torch.empty(max(16, ops.attention_paged_workspace_bytes(B * T, B, nh, nkv, hd, T, 64, 0, torch.bfloat16)),
+                     dtype=torch.uint8, device=DEV)
+    kv = lambda i: qkv[:, :, (nh + i * nkv) * hd: (nh + (i + 1) * nkv) * hd].view(layers, B * T, nkv, hd)
+
+    def step():
+        ops.page_tables(seq_len, row0, table, held, free, top, ps, B * T, st, slots=slots)
+        ops.kv_write_paged(kv(0), kv(1), pools[0], pools[1], slots, st)
+        ops.tree_attention_paged(qkv[1, :, : nh * hd].view(B * T, nh, hd), pools[0][1], pools[1][1], table, row0, seq_len,
+                                 hd ** -0.5, T, 64, st, bits=bits, workspace=ws, out=out)
+        ops.kv_compact_paged(pools[0], pools[1], table, seq_len, acc, st)
+        seq_len.add_(acc[:, 0])
+
+    step()  # loads the kernels
+    keep = [torch.zeros((B, 0, nkv, hd), dtype=torch.float64, device=DEV) for _ in range(2)]
+    seq_len.zero_(), held.zero_(), top.fill_(pages), table.fill_(-1)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    for rep in range(6):
+        qkv.copy_(torch.randn(qkv.shape, generator=gen).to(torch.bfloat16))
+        out.fill_(9.0)
+        g.replay()
+        torch.cuda.synchronize()
+        new = [kv(i)[1].view(B, T, nkv, hd).double() for i in range(2)]
+        for b in range(B):
+            k, v = (torch.cat([keep[i][b], new[i][b]]) for i in range(2))
+            n = keep[0].shape[1]
+            see = torch.cat([torch.ones((T, n), dtype=torch.bool, device=DEV),
+                             ((bits[b * T: (b + 1) * T] >> torch.arange(T, device=DEV)) & 1) == 1], 1)
+            for h in range(nh):
+                q = qkv[1, b * T: (b + 1) * T, h * hd: (h + 1) * hd].double()
+                s = (q @ k[:, h // 4].t().contiguous() * hd ** -0.5).masked_fill(~see, -math.inf)
+                w = torch.softmax(s, 1)
+                ref, mag = w @ v[:, h // 4], w @ v[:, h // 4].abs()
+                got = out[b * T: (b + 1) * T, h * hd: (h + 1) * hd].double()
+                u = torch.finfo(torch.bfloat16).eps / 2
+                assert bool(((got - ref).abs() <= u * ref.abs() + (u + 2.0 ** -13) * mag).all()), (rep, b, h)
+        keep = [torch.cat([keep[i], new[i][:, [0, 3, 4]]], 1) for i in range(2)]
+        assert seq_len.tolist() == [3 * (rep + 1)] * B and int(st.item()) == 0
