@@ -173,6 +173,7 @@ SIGNATURES: dict[str, tuple] = {
     "pe_kv_compact_paged": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, i64, C.c_int, vp, i64, i64, C.c_int,
                                       vp, i64, vp, C.c_int, vp, vp]),
     "pe_attention_paged_workspace_bytes": (i64, [i64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, i64, i64, C.c_int]),
+    "pe_attention_paged_reserve_bytes": (i64, [i64, C.c_int, C.c_int, C.c_int, C.c_int]),
     "pe_tree_attention_paged": (C.c_int, [C.POINTER(PagedAttentionArgs), vp]),
     "pe_loop_commit": (C.c_int, [vp, C.c_int, vp, vp, C.c_int, vp, i64, C.c_int, vp, vp, vp, i64, vp, vp, C.c_int,
                                  vp, vp, vp, vp]),

@@ -93,5 +93,6 @@ __device__ __forceinline__ int prefix_parts_of(const PagedPrefix& p, uint32_t bl
 // pe_paged_attn.hip: the call on the matrix cores (bf16 / fp16, hd 64 or 128).
 PE_INTERNAL int64_t pe_internal_paged_mfma_bytes(int64_t M, int batch, int nh, int nkv, int hd, int max_rows,
                                                  int64_t max_len, int64_t prefix_len);
+PE_INTERNAL int64_t pe_internal_paged_mfma_reserve(int64_t M, int nh, int nkv, int hd);
 PE_INTERNAL int pe_internal_paged_mfma(const PagedAttn& a, int dtype, void* workspace, int64_t workspace_bytes,
                                        hipStream_t st);

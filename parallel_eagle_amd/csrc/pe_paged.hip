@@ -655,6 +655,11 @@ extern "C" int pe_tree_attention_paged(const pe_paged_attention_args* p, void* s
   return pe_internal_tree_attention_paged(p, 0, (hipStream_t)stream);
 }
 
+extern "C" int64_t pe_attention_paged_reserve_bytes(int64_t M, int nh, int nkv, int hd, int dtype) {
+  if (M <= 0 || nh <= 0 || nkv <= 0 || nh % nkv || !mfma_fits(hd, dtype)) return 0;
+  return pe_internal_paged_mfma_reserve(M, nh, nkv, hd);
+}
+
 int pe_internal_tree_attention_paged(const pe_paged_attention_args* p, int out_units, hipStream_t st) {
   if (!p) return PE_ERR_ARG;
   const int es = esize(p->dtype), psl = page_log2(p->page_size);
@@ -667,7 +672,8 @@ int pe_internal_tree_attention_paged(const pe_paged_attention_args* p, int out_u
       p->max_len < p->prefix_len || p->max_len >= (int64_t(1) << 30) || p->num_pages <= 0 ||
       p->num_pages >= (int64_t(1) << 31) || p->ld_table <= 0 || p->table_cols <= 0 || p->ld_table < p->table_cols ||
       p->table_cols >= (int64_t(1) << 31) || p->ld_q < (int64_t)p->nh * p->hd || p->ld_out < (int64_t)p->nh * p->hd ||
-      p->window < 0 || !(p->softcap >= 0.f) || !(p->scale > 0.f))
+      p->window < 0 || !(p->softcap >= 0.f && p->softcap < INFINITY) || !(p->scale > 0.f && p->scale < INFINITY) ||
+      (int64_t)p->nkv * p->page_size * p->hd * es >= (int64_t(1) << 32))
     return PE_ERR_ARG;
   if (p->prefix_len > 0 && (!p->prefix_table || p->prefix_pages < ((p->prefix_len - 1) >> psl) + 1)) return PE_ERR_ARG;
   if (p->mask_mode == PE_MASK_TREE) {

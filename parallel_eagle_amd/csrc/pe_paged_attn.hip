@@ -244,13 +244,10 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
 
   // the lane's LDS offsets: K row ln of a 32-key block, and V's transposed reads
   const int qg = lane >> 4, jl = lane & 15, vrow = 4 * (qg >> 1) + (jl >> 2), vcol = 16 * (qg & 1) + 4 * (jl & 3);
-  uint32_t k_at[HD / 16], v_at[2][OB];
-#pragma unroll
-  for (int j = 0; j < HD / 16; ++j) k_at[j] = lds_at<HD>(ln, 2 * j + g);
-#pragma unroll
-  for (int h = 0; h < OB; ++h)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) v_at[e][h] = lds_at<HD>(vrow + 8 * e, (32 * (hb + h) + vcol) >> 3) + (vcol & 7) * 2;
+  // (the chunk's upper bits, 2 j of K and 4 h of V, meet only zeros of the rest: one exclusive or each)
+  const uint32_t k_at = lds_at<HD>(ln, g);
+  const uint32_t v_at[2] = {(lds_at<HD>(vrow, vcol >> 3) ^ (hb << 6)) + (vcol & 7) * 2,
+                            (lds_at<HD>(vrow + 8, vcol >> 3) ^ (hb << 6)) + (vcol & 7) * 2};
 
   if (s0 < s1) ask(s0);
   __syncthreads();  // the buffers' last readers are done
@@ -274,29 +271,32 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
     const bool pre = s < k.pre_steps;
     const int kb0 = (pre ? s : s - k.pre_steps) * C::SK, kpos = kb0 + (pre ? 0 : k.base);  // key 0 of the step
     if (!live || (!pre && kb0 > k.last)) continue;  // wave-uniform: the tile sees no key of this step
-    const uint8_t* kbp = smem + (s % C::ST) * C::kStep;
-    const uint8_t* vbp = kbp + C::kHalf;
+    const uint32_t stage = (s % C::ST) * C::kStep;
+    const uint32_t ks = stage + k_at, vs[2] = {stage + v_at[0], stage + v_at[1]};
     // products on two chains of accumulators at least (a chain alone waits for each product)
     constexpr int kChains = SB > 1 ? SB : 2;
     f32x16_t sc[kChains];
     // Fragments in groups of LDS reads, kAhead groups ahead of the products that
     // use them: kS groups of four products of S, then 2 SB groups (16 keys each)
-    // of V, whose first kAhead are read before the softmax.
-    constexpr int kS = SB * HD / 64, kAll = kS + 2 * SB, kAhead = 2, kF = kAhead + 1;
+    // of V, whose first kAhead are read before the softmax. (One group ahead
+    // where other scores leave 64 keys of 128 dims no registers.)
+    constexpr int kS = SB * HD / 64, kAll = kS + 2 * SB, kAhead = MOD && HD == 128 && SB == 2 ? 1 : 2, kF = kAhead + 1;
     u32x4_t f[kF][4];
     auto read = [&](int gr) {
       if (gr < kS) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int at = 4 * gr + i;  // product SB j + sb
-          f[gr % kF][i] = *(const u32x4_t*)(kbp + k_at[at / SB] + (at % SB) * 32 * HD * 2);
+          f[gr % kF][i] = *(const u32x4_t*)(smem + (ks ^ ((at / SB) << 5)) + (at % SB) * 32 * HD * 2);
         }
       } else if (gr < kAll) {
 #pragma unroll
         for (int h = 0; h < OB; ++h) {
-          const uint8_t* vq = vbp + (gr - kS) * 16 * HD * 2;
-          const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v_t*)(vq + v_at[0][h])));
-          const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v_t*)(vq + v_at[1][h])));
+          const uint8_t* vq = smem + C::kHalf + (gr - kS) * 16 * HD * 2;
+          const uint2 x = __builtin_bit_cast(
+              uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v_t*)(vq + (vs[0] ^ (h << 6)))));
+          const uint2 y = __builtin_bit_cast(
+              uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v_t*)(vq + (vs[1] ^ (h << 6)))));
           f[gr % kF][h] = u32x4_t{x.x, x.y, y.x, y.y};
         }
       }
@@ -917,10 +917,9 @@ __device__ __forceinline__ void seq_item(const PagedAttn& a, const PagedPrefix& 
 // Many rows over a long prefix: eight tiles (256 rows) on every K / V byte, one
 // workgroup per CU.
 template <int HD> using Wide = Cfg<HD, 8, 1, 2, 4>;
-// Four waves, 64 KiB of LDS, two workgroups per CU. (Other scores of 128-dim
-// heads by 32 keys: 64 leave their registers no room, and a spilled one is
-// reloaded behind the loads in flight.)
-template <int HD, bool MOD> using Four = Cfg<HD, 4, 1, MOD && HD == 128 ? 1 : 2, HD == 128 && !MOD ? 2 : 4>;
+// Four waves, 64 KiB of LDS, two workgroups per CU. (Steps of 32 keys instead of
+// 64 for 128-dim heads: level for plain scores, 12% slower for capped ones.)
+template <int HD> using Four = Cfg<HD, 4, 1, 2, HD == 128 ? 2 : 4>;
 template <int HD> using Two = Cfg<HD, 4, 2, HD == 128 ? 1 : 2, 4>;
 template <int HD> using One = Cfg<HD, 4, HD == 128 ? 4 : 2, HD == 128 ? 1 : 2, 4>;
 
@@ -937,19 +936,19 @@ __global__ __launch_bounds__(512, 2) void paged_prefix_kernel(PagedAttn a, Paged
 template <int DT, int HD, bool MOD>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttn a, PagedPrefix pp, PagedParts parts, PagedSeqs sq,
                                                             uint32_t n_pre, int pre_kind) {
-  constexpr int kSmem = Two<HD>::kSmem > Four<HD, MOD>::kSmem ? Two<HD>::kSmem : Four<HD, MOD>::kSmem;
+  constexpr int kSmem = Two<HD>::kSmem > Four<HD>::kSmem ? Two<HD>::kSmem : Four<HD>::kSmem;
   static_assert(One<HD>::kSmem <= kSmem, "one ring for every kind");
   __shared__ __align__(1024) uint8_t smem[kSmem];
   __shared__ int s_npos[MOD ? 64 * PE_TREE_MAX_WORDS : 1];
   __shared__ int s_lo[4];
   if (blockIdx.x < n_pre) {
     const uint32_t w = xcd_item(blockIdx.x, n_pre);
-    if (pre_kind == 4) prefix_share<DT, Four<HD, MOD>, MOD>(a, pp, parts, w, smem, s_lo);
+    if (pre_kind == 4) prefix_share<DT, Four<HD>, MOD>(a, pp, parts, w, smem, s_lo);
     else if (pre_kind == 2) prefix_share<DT, Two<HD>, MOD>(a, pp, parts, w, smem, s_lo);
     else prefix_share<DT, One<HD>, MOD>(a, pp, parts, w, smem, s_lo);
   } else {
     const uint32_t item = blockIdx.x - n_pre;
-    if (sq.kind == 4) seq_item<DT, Four<HD, MOD>, MOD>(a, pp, parts, sq, item, smem, s_npos, s_lo);
+    if (sq.kind == 4) seq_item<DT, Four<HD>, MOD>(a, pp, parts, sq, item, smem, s_npos, s_lo);
     else if (sq.kind == 2) seq_item<DT, Two<HD>, MOD>(a, pp, parts, sq, item, smem, s_npos, s_lo);
     else seq_item<DT, One<HD>, MOD>(a, pp, parts, sq, item, smem, s_npos, s_lo);
   }
@@ -1011,8 +1010,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefi
 
 // ------------------------------------------------------------------ plans
 constexpr int kCus = 256;
-constexpr int kSeqWgs = 1024, kSlimWgs = 2048, kMinSplit = 64, kSplitRows = 2, kPrefixSteps = 4, kFusedPre = 256, kFoldKeys = 64;
-constexpr int64_t kWideUnits = 4096;
+constexpr int64_t kSeqWgs = 1024, kSlimWgs = 2048, kMinSplit = 64, kSplitRows = 2, kPrefixSteps = 4, kFusedPre = 256, kFoldKeys = 64;
+constexpr int64_t kWideUnits = 32768, kSplitTiles = 10240;
 
 // A launch's workgroups: which configuration, row tiles per block and how many
 // blocks hold `tiles` row tiles in equal shares.
@@ -1026,7 +1025,7 @@ Shape shape_of(int64_t tiles, int most) {
   return {most == 8 ? 8 : each > 2 ? 4 : each, each, blocks};
 }
 // Keys of a step (the configurations above).
-int step_keys(const Shape& s, int hd, bool mod) { return hd == 64 || s.kind == 8 || (s.kind == 4 && !mod) ? 64 : 32; }
+int step_keys(const Shape& s, int hd) { return hd == 64 || s.kind >= 4 ? 64 : 32; }
 
 struct Plan {
   PagedPrefix pp;
@@ -1037,8 +1036,7 @@ struct Plan {
   int64_t units, items, pre_wgs, o_bytes, ml_bytes;
 };
 
-Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int64_t max_len, int64_t prefix_len,
-               bool mod) {
+Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int64_t max_len, int64_t prefix_len) {
   Plan p;
   const int G = nh / nkv;
   const int64_t tiles = (M * G + 31) / 32;
@@ -1048,17 +1046,17 @@ Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int6
   p.pt.pre_parts = p.pre_kind = 0;
   p.wide = false;
   const Shape seq = shape_of(((int64_t)max_rows * G + 31) / 32, 4);
-  const int step = step_keys(seq, hd, mod);
+  const int step = step_keys(seq, hd);
   const int64_t own_keys = max_len - prefix_len + max_rows;
   const bool fold = prefix_len <= std::max<int64_t>(kFoldKeys, max_rows * G);
   const int64_t pre_steps = fold ? (prefix_len + step - 1) / step : 0;
   if (!fold) {
     const int64_t s64 = (prefix_len - 1) / 64 + 1;
     // many rows over many keys: the wide blocks' own launch
-    p.wide = tiles > 4 && tiles * s64 * nkv >= kWideUnits * 8;
+    p.wide = tiles > 4 && tiles * s64 * nkv >= kWideUnits;
     const Shape pre = shape_of(tiles, p.wide ? 8 : 4);
     p.pre_kind = pre.kind;
-    const int64_t steps = (prefix_len - 1) / step_keys(pre, hd, mod) + 1, blocks = nkv * pre.blocks;
+    const int64_t steps = (prefix_len - 1) / step_keys(pre, hd) + 1, blocks = nkv * pre.blocks;
     if (p.wide) {
       p.units = blocks * steps;
       const int64_t per = (p.units + kCus - 1) / kCus;
@@ -1068,7 +1066,7 @@ Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int6
       // the sequences' steps of 64 keys per place, half of the longest on average: the
       // prefix's shares run beside them, and fewer parts are cheaper to join
       const int64_t beside = batch * nkv * seq.blocks * own_keys / (64 * 2 * 2 * kCus);
-      const int64_t least = std::max<int64_t>(kPrefixSteps, beside * 64 / step_keys(pre, hd, mod));
+      const int64_t least = std::max<int64_t>(kPrefixSteps, beside * 64 / step_keys(pre, hd));
       const int64_t k = std::max<int64_t>(1, std::min<int64_t>(kFusedPre / blocks, steps / least));
       const int64_t per = (steps + k - 1) / k, parts = (steps + per - 1) / per;
       p.units = blocks * per * parts;
@@ -1081,8 +1079,12 @@ Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int6
   const int64_t steps = pre_steps + (own_keys - 1) / step + 1;
   const int64_t wgs = batch * nkv * seq.blocks;
   const int64_t blk_rows = std::min<int64_t>(32 * seq.tiles, (int64_t)max_rows * G);
+  // splits fill the machine about twice (few rows: four times, their parts are
+  // small), each no shorter than kMinSplit keys or kSplitRows keys a row; a batch
+  // of many padding rows has its parts limited
   const int64_t ns = std::max<int64_t>(
-      1, std::min<int64_t>((blk_rows > 64 ? kSeqWgs : kSlimWgs) / wgs, steps * step / std::max<int64_t>(kMinSplit, kSplitRows * blk_rows)));
+      1, std::min({(blk_rows > 64 ? kSeqWgs : kSlimWgs) / wgs,
+                   steps * step / std::max<int64_t>(kMinSplit, kSplitRows * blk_rows), kSplitTiles / (nkv * tiles)}));
   const int64_t split_steps = (steps + ns - 1) / ns, nsplit = (steps + split_steps - 1) / split_steps;
   p.items = wgs * nsplit;
   const bool direct = fold || (p.wide && p.pt.pre_parts <= 3);
@@ -1116,14 +1118,22 @@ int launch_all(const Plan& p, const PagedAttn& a, hipStream_t st) {
 
 int64_t pe_internal_paged_mfma_bytes(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int64_t max_len,
                                      int64_t prefix_len) {
-  const Plan p = make_plan(M, batch, nh, nkv, hd, max_rows, max_len, prefix_len, false);
-  const Plan m = make_plan(M, batch, nh, nkv, hd, max_rows, max_len, prefix_len, true);
-  return std::max(p.o_bytes + p.ml_bytes, m.o_bytes + m.ml_bytes);
+  const Plan p = make_plan(M, batch, nh, nkv, hd, max_rows, max_len, prefix_len);
+  return p.o_bytes + p.ml_bytes;
+}
+
+// Row tiles x KV heads x parts that no plan of up to M rows passes: the wide
+// launch's parts, of at most 256 / (nkv blocks) + 2 per block of eight tiles, or
+// the shared launch's, of which there are as many as workgroups (four tiles
+// each) or one; and the splits (make_plan's limit).
+int64_t pe_internal_paged_mfma_reserve(int64_t M, int nh, int nkv, int hd) {
+  const int64_t tiles = nkv * ((M * (nh / nkv) + 31) / 32);
+  return (2 * tiles + 8 * kCus + std::max(tiles, kSplitTiles)) * (32 * hd * 4 + 32 * 8);
 }
 
 int pe_internal_paged_mfma(const PagedAttn& a, int dtype, void* workspace, int64_t workspace_bytes, hipStream_t st) {
   const bool mod = a.softcap > 0.f || a.slopes || a.window > 0;
-  Plan p = make_plan(a.M, a.batch, a.nh, a.nkv, a.hd, a.max_rows, a.max_len, a.prefix_len, mod);
+  Plan p = make_plan(a.M, a.batch, a.nh, a.nkv, a.hd, a.max_rows, a.max_len, a.prefix_len);
   if (p.o_bytes > 0 && (!workspace || workspace_bytes < p.o_bytes + p.ml_bytes)) return PE_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 15) return PE_ERR_ARG;
   // rows and work units are counted in 32 bits

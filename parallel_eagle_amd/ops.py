@@ -537,9 +537,15 @@ def kv_compact_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: to
 
 def attention_paged_workspace_bytes(m: int, batch: int, nh: int, nkv: int, hd: int, max_rows: int, max_len: int,
                                     prefix_len: int, dtype: torch.dtype) -> int:
-    """Bytes of workspace a ``tree_attention_paged`` call of these sizes needs (no initial value)."""
+    """Bytes of workspace a ``tree_attention_paged`` call of exactly these sizes needs (no initial value; a smaller
+    call may need more, see ``attention_paged_reserve_bytes``)."""
     return int(lib().pe_attention_paged_workspace_bytes(m, batch, nh, nkv, hd, max_rows, max_len, prefix_len,
                                                         dcode(dtype)))
+
+
+def attention_paged_reserve_bytes(m: int, nh: int, nkv: int, hd: int, dtype: torch.dtype) -> int:
+    """Bytes of workspace that hold every ``tree_attention_paged`` call of up to m rows with these heads."""
+    return int(lib().pe_attention_paged_reserve_bytes(m, nh, nkv, hd, dcode(dtype)))
 
 
 def tree_attention_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,

@@ -2,6 +2,7 @@
 launched: the pointers are never read) and what their wrappers raise."""
 
 import ctypes as C
+import random
 
 import pytest
 import torch
@@ -37,7 +38,8 @@ REFUSED = [dict(q=None), dict(k_pool=None), dict(v_pool=None), dict(out=None), d
            dict(page_size=2048), dict(batch=0), dict(nkv=3), dict(nkv=0), dict(hd=0), dict(hd=264), dict(M=-1),
            dict(max_rows=-1), dict(prefix_len=-1), dict(max_len=19), dict(max_len=1 << 30), dict(num_pages=0),
            dict(table_cols=0), dict(ld_table=3), dict(ld_q=1023), dict(ld_out=1016), dict(window=-1), dict(softcap=-1.0),
-           dict(softcap=float("nan")), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(mask_mode=2),
+           dict(softcap=float("nan")), dict(softcap=float("inf")), dict(scale=float("inf")),
+           dict(nkv=1 << 14, nh=1 << 14, page_size=1024, ld_q=1 << 21, ld_out=1 << 21), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(mask_mode=2),
            dict(words=0), dict(prefix_table=None), dict(prefix_pages=1), dict(window=4, positions=None),
            dict(slopes=64, positions=None), dict(workspace=72)]
 
@@ -67,14 +69,22 @@ def test_workspace_bytes_of_calls_that_are_refused_or_need_none(lib):
     assert f(10, 2, 8, 2, 128, 8, 10, 20, 1) == 0
 
 
-@pytest.mark.parametrize("m,batch,rows,length,prefix", [(1, 1, 1, 100, 0), (26, 1, 26, 5000, 4000), (416, 16, 26, 3200, 2048),
-                                                        (1664, 64, 26, 9192, 8192), (700, 1, 700, 1000, 300)])
+@pytest.mark.parametrize("heads", [(32, 32), (40, 8), (16, 16), (8, 1)])
 @pytest.mark.parametrize("hd", [64, 128])
-def test_workspace_grows_with_the_sizes_that_a_call_bounds(lib, m, batch, rows, length, prefix, hd):
-    """Parts are counted in whole row tiles: no less for more heads, and a call of the same sizes fits."""
-    f = lambda nh, nkv: lib.pe_attention_paged_workspace_bytes(m, batch, nh, nkv, hd, rows, length, prefix, 1)
-    assert f(8, 8) >= 0 and f(16, 8) >= 0
-    assert f(8, 8) % 8 == 0
+def test_a_reserve_holds_every_smaller_call(lib, heads, hd):
+    rng = random.Random(hd + heads[0])
+    nh, nkv = heads
+    for _ in range(400):
+        top = round(2 ** rng.uniform(0, 14))
+        room = lib.pe_attention_paged_reserve_bytes(top, nh, nkv, hd, _lib.PE_DTYPE_BF16)
+        m = rng.randint(1, top)
+        batch = rng.randint(1, min(m, 65535))
+        rows = rng.choice([-(-m // batch), rng.randint(1, m)])
+        prefix = rng.choice([0, rng.randint(1, 100), round(2 ** rng.uniform(0, 17))])
+        length = prefix + rng.choice([0, round(2 ** rng.uniform(0, 17))])
+        need = lib.pe_attention_paged_workspace_bytes(m, batch, nh, nkv, hd, min(rows, 65535), length, prefix,
+                                                      _lib.PE_DTYPE_BF16)
+        assert need <= room, (top, m, batch, rows, length, prefix)
 
 
 def tables(lib, **kw):
