@@ -738,13 +738,16 @@ __device__ __forceinline__ void prefix_share(const PagedAttn& a, const PagedPref
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int ln = lane & 31, g = lane >> 5, tile = wave / C::DS, hb = (wave % C::DS) * C::OB;
   const uint32_t G = (uint32_t)(a.nh / a.nkv), R = (uint32_t)a.M * G;
-  const uint32_t uend = min(pp.total, (w + 1) * pp.per);
+  // its pieces of blocks from the last to the first: a piece that ends its share
+  // starts at key 0 and one that starts it ends at the last key, so workgroups
+  // walk the keys at the same time, from one copy in their XCD's L2
+  const uint32_t u0 = w * pp.per;
   bool bad = false;
-  for (uint32_t u = w * pp.per; u < uend;) {
-    const uint32_t x = u / pp.steps;
-    const int s0 = (int)(u - x * pp.steps);
-    const uint32_t past = min(pp.steps, s0 + (uend - u));  // a block's last steps may be beyond its keys
-    u += past - s0;
+  for (uint32_t u = min(pp.total, u0 + pp.per); u > u0;) {
+    const uint32_t x = (u - 1) / pp.steps, first_u = max(u0, x * pp.steps);
+    const int s0 = (int)(first_u - x * pp.steps);
+    const uint32_t past = u - x * pp.steps;  // a block's last steps may be beyond its keys
+    u = first_u;
     const int s1 = min((int)past, ((int)a.prefix_len - 1) / C::SK + 1);
     const int kvh = (int)(x / pp.nblk);
     const uint32_t blk0 = (x - kvh * pp.nblk) * pp.block_rows, row0 = blk0 + 32 * tile;
@@ -788,6 +791,7 @@ __device__ __forceinline__ void prefix_share(const PagedAttn& a, const PagedPref
 // prefix's parts of its rows to its own (an earlier launch wrote them, and they
 // are few) and writes the output; otherwise its result is a part as well and
 // paged_join_kernel writes the output.
+constexpr int kDirectParts = 3;  // the most parts a sequence's workgroup joins itself
 struct PagedSeqs {
   uint32_t items, nblk, block_rows;
   int split_steps, pre_steps, step, nsplit, kind, direct;
@@ -1087,7 +1091,7 @@ Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int6
                    steps * step / std::max<int64_t>(kMinSplit, kSplitRows * blk_rows), kSplitTiles / (nkv * tiles)}));
   const int64_t split_steps = (steps + ns - 1) / ns, nsplit = (steps + split_steps - 1) / split_steps;
   p.items = wgs * nsplit;
-  const bool direct = fold || (p.wide && p.pt.pre_parts <= 3);
+  const bool direct = fold || (p.wide && p.pt.pre_parts <= kDirectParts);
   p.sq = PagedSeqs{(uint32_t)p.items, (uint32_t)seq.blocks, (uint32_t)(32 * seq.tiles), (int)split_steps, (int)pre_steps,
                    step, (int)nsplit, seq.kind, direct};
   p.join = nsplit > 1 || !direct;
