@@ -442,6 +442,10 @@ __device__ __forceinline__ void attend(const PagedAttn& a, uint8_t* smem, const 
 // loads issued after those are one step's, so two steps are in flight.
 //
 // LDS reads run two groups of four matrix instructions ahead of their use.
+// 14b, 64 trees of 26 nodes over 8192 shared keys (279 GFLOP of products with the
+// prefix): 249 us, 1.12 PFLOP/s, where a large matrix product of the library
+// reaches 1.21 on the same card; one barrier a step took 19 us more on the whole
+// call, phases without s_setprio 4 us more, without the slack below 9 us.
 // A row's running maximum follows its block's only when it is passed by more
 // than 2^8 (kSlack): O and l are sums of the same 2^(s - m), whichever m, and the
 // weights, at most 2^8, lose nothing in fp32 nor when rounded (fp16's largest
@@ -791,7 +795,10 @@ __device__ __forceinline__ void prefix_share(const PagedAttn& a, const PagedPref
 // prefix's parts of its rows to its own (an earlier launch wrote them, and they
 // are few) and writes the output; otherwise its result is a part as well and
 // paged_join_kernel writes the output.
-constexpr int kDirectParts = 3;  // the most parts a sequence's workgroup joins itself
+// The most parts of the prefix that a sequence's workgroup joins itself (14b,
+// trees of 26 nodes: 64 over 8192 keys, 3 parts, 326, and 345 with the join's
+// launch; 16 over 8192, 6 parts, 94 / 104; 16 over 16384, 8 parts, 165 / 170).
+constexpr int kDirectParts = 8;
 struct PagedSeqs {
   uint32_t items, nblk, block_rows;
   int split_steps, pre_steps, step, nsplit, kind, direct;
@@ -960,7 +967,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttn a, PagedPr
 
 // Joins the parts: one thread per (row, four dims), 32 rows x 32 dims a block
 // (512 contiguous bytes of a part per load), the prefix's parts first, then the
-// splits in key order.
+// splits in key order. Bound by latency (7 - 10 us at 10 - 60 MB of parts, the
+// launch included), so kAhead parts are asked for at once; eight at once were
+// level at best and cost registers.
 template <int DT, int HD>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefix pp, PagedParts parts, PagedSeqs sq) {
   const int b = blockIdx.z, kvh = blockIdx.y;
@@ -1013,9 +1022,43 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, PagedPrefi
 }
 
 // ------------------------------------------------------------------ plans
+// The rules below choose among forms that compute the same thing, by counts of
+// rows, keys and workgroups. Both sides of each were measured (us a call, all
+// launches; "14b": 40 query heads on 8 KV heads of 128 dims, "7b": 32 on 32).
 constexpr int kCus = 256;
-constexpr int64_t kSeqWgs = 1024, kSlimWgs = 2048, kMinSplit = 64, kSplitRows = 2, kPrefixSteps = 4, kFusedPre = 256, kFoldKeys = 64;
-constexpr int64_t kWideUnits = 32768, kSplitTiles = 10240;
+// A prefix of up to this many keys, or of as many as a sequence has rows, is
+// read with each sequence's own keys: its parts would cost more than that.
+// 7b, 12 sequences of up to 18 rows, 10 shared keys: 10.8, as a share of its own
+// 15.8; 14b, 7 of 270 rows, 12 keys: 44.2 / 67.3; 59 of 6 rows, 23 keys: 35.2 /
+// 45.7. Past the rule it loses: four times as many keys as rows, 14b, 43
+// sequences, 279 keys: 73.6 folded / 68.5; up to 128 keys, 2 sequences, 93: 15.2 / 13.4.
+constexpr int64_t kFoldKeys = 64;
+// Wide blocks in a launch of their own from this many (32-row tile, 64-key step,
+// KV head) units on: 14b, trees of 26 nodes, 64 over 8192 shared keys (266 240
+// units): 326 with the wide launch, 449 without; 16 over 8192 (66 560): 94 / 185;
+// 32 over 3000 (48 880): 101 / 107. Below, the shared launch, where the
+// sequences' loads fill the prefix's waits: 32 over 1500 (24 960) 73.6 / 66.0; 7b,
+// 16 over 3000 (19 552) 68.1 / 54.9, over 2048 (13 312) 71.7 / 63.5.
+constexpr int64_t kWideUnits = 32768;
+// Workgroups of the prefix in the shared launch, one of the two places of each
+// CU. 7b, 16 trees over 2048 keys: 63.2; 128 of them 65.2, 384 69.6, 512 66.5;
+// four chunks of 128 rows with slopes: 53.0, 57.4 (128), 63.5 (512).
+constexpr int64_t kFusedPre = 256;
+// The least steps of a prefix share. 27 sequences of one token: 16.4; 2 steps
+// 21.1 (more parts to join); 8 steps lose on short prefixes, 26.2 / 19.3.
+constexpr int64_t kPrefixSteps = 4;
+// Workgroups that the splits of the sequences' keys are to reach: 1024 where a
+// workgroup has more than 64 rows (14b, 8 capped sequences with a window: 62;
+// 512: 81; 1536: 66), 2048 where it has fewer, whose parts are smaller (14b, 64
+// one-token sequences: 52.3; 1024: 55.1; 4096: 57.7).
+constexpr int64_t kSeqWgs = 1024, kSlimWgs = 2048;
+// The least keys of a split, and the least per row of its block: 64 (one 14b
+// sequence of 428 keys: 12.0; 128: 13.2) and 2 (the capped sequences above:
+// 57.4; 8: 78.8; chunks with slopes 45.2 / 52.0).
+constexpr int64_t kMinSplit = 64, kSplitRows = 2;
+// Row tiles x KV heads x splits at most: bounds the parts of a batch that is
+// mostly padding.
+constexpr int64_t kSplitTiles = 10240;
 
 // A launch's workgroups: which configuration, row tiles per block and how many
 // blocks hold `tiles` row tiles in equal shares.
@@ -1073,10 +1116,21 @@ Plan make_plan(int64_t M, int batch, int nh, int nkv, int hd, int max_rows, int6
       const int64_t least = std::max<int64_t>(kPrefixSteps, beside * 64 / step_keys(pre, hd));
       const int64_t k = std::max<int64_t>(1, std::min<int64_t>(kFusedPre / blocks, steps / least));
       const int64_t per = (steps + k - 1) / k, parts = (steps + per - 1) / per;
-      p.units = blocks * per * parts;
-      p.pp = PagedPrefix{(uint32_t)p.units, (uint32_t)per, (uint32_t)(per * parts), (uint32_t)pre.blocks,
-                         (uint32_t)(32 * pre.tiles)};
-      p.pt.pre_parts = (int)parts;
+      if (2 * blocks > kFusedPre && 4 * blocks * parts < 3 * kFusedPre) {
+        // a share per block would leave over a quarter of the places empty: shares that cross
+        // blocks (14b, 16 trees of 26 nodes over 2048 keys, 136 blocks: 46.1, 60.8 with a share
+        // each; where whole shares fill the places they are as good or better, 61.3 / 65.6)
+        const int64_t even = std::max(least, (blocks * steps + kFusedPre - 1) / kFusedPre);
+        p.units = blocks * steps;
+        p.pp = PagedPrefix{(uint32_t)p.units, (uint32_t)even, (uint32_t)steps, (uint32_t)pre.blocks,
+                           (uint32_t)(32 * pre.tiles)};
+        p.pt.pre_parts = (int)((steps - 1) / even) + 2;
+      } else {
+        p.units = blocks * per * parts;
+        p.pp = PagedPrefix{(uint32_t)p.units, (uint32_t)per, (uint32_t)(per * parts), (uint32_t)pre.blocks,
+                           (uint32_t)(32 * pre.tiles)};
+        p.pt.pre_parts = (int)parts;
+      }
     }
     p.pre_wgs = (p.units + p.pp.per - 1) / p.pp.per;
   }
@@ -1129,7 +1183,8 @@ int64_t pe_internal_paged_mfma_bytes(int64_t M, int batch, int nh, int nkv, int 
 // Row tiles x KV heads x parts that no plan of up to M rows passes: the wide
 // launch's parts, of at most 256 / (nkv blocks) + 2 per block of eight tiles, or
 // the shared launch's, of which there are as many as workgroups (four tiles
-// each) or one; and the splits (make_plan's limit).
+// each), one, or up to three of fewer than 768 tiles; and the splits (make_plan's
+// limit).
 int64_t pe_internal_paged_mfma_reserve(int64_t M, int nh, int nkv, int hd) {
   const int64_t tiles = nkv * ((M * (nh / nkv) + 31) / 32);
   return (2 * tiles + 8 * kCus + std::max(tiles, kSplitTiles)) * (32 * hd * 4 + 32 * 8);

@@ -245,6 +245,16 @@ def test_many_rows_over_a_long_prefix(heads, dtype, seqs, prefix, cap, window, b
     c.check(c.run())
 
 
+@pytest.mark.parametrize("cap,window,bias", [(0.0, 0, False), (40.0, 0, True), (0.0, 300, False)])
+@pytest.mark.parametrize("heads,dtype,seqs,prefix", [((40, 8, 128), torch.bfloat16, 16, 701), ((32, 32, 64), torch.float16, 20, 660)],
+                         ids=["14b", "64"])
+def test_prefix_shares_that_cross_row_blocks(heads, dtype, seqs, prefix, cap, window, bias):
+    """136 and 160 row blocks of the prefix, fewer than the 256 workgroups that share them."""
+    c = Case(heads, [26] * seqs, [(37 * i) % 90 for i in range(seqs)], prefix, page=32, dtype=dtype, seed=13, cap=cap,
+             window=window, bias=bias)
+    c.check(c.run())
+
+
 @pytest.mark.parametrize("heads,dtype", LAYOUTS[:4], ids=IDS[:4])
 @pytest.mark.parametrize("prefix", [0, 40])
 def test_rows_that_see_nothing_are_zero(heads, dtype, prefix):
