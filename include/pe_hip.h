@@ -396,9 +396,10 @@ int pe_kv_compact_paged(void* k_pool, void* v_pool, int L, int nkv, int hd, int 
  * unnormalised probabilities to the type for the PV product, as
  * pe_tree_attention does. K of a key that a row does not see may hold anything;
  * V of the cached keys and of the new rows must be finite (the matrix cores add
- * zero times the V of a key that a row does not see but others may). Any hd <= 256; bf16 / fp16 with hd 64 or 128 run on the
- * matrix cores where q, the pools and out are 16-byte aligned with ld_q and
- * ld_out multiples of 8. A page of all KV heads is smaller than 4 GiB. */
+ * zero times the V of a key that a row does not see but others may). Any hd <=
+ * 256; bf16 / fp16 with hd 64 or 128 run on the matrix cores where q, the pools
+ * and out are 16-byte aligned with ld_q and ld_out multiples of 8. A page of all
+ * KV heads is smaller than 4 GiB. */
 typedef struct pe_paged_attention_args {
   const void* q;       /* [M][nh][hd], rows ld_q elements apart */
   const void* k_pool;  /* [num_pages][nkv][page_size][hd] */
@@ -423,10 +424,11 @@ typedef struct pe_paged_attention_args {
   int32_t _reserved;
 } pe_paged_attention_args;
 /* Workspace for a call of exactly these sizes (a smaller call may need more: it
- * is split further), and for every call of up to M rows with these heads. */
-int64_t pe_attention_paged_reserve_bytes(int64_t M, int nh, int nkv, int hd, int dtype);
+ * is split further), and for every call of up to M rows with these heads. Calls
+ * that may run at the same time need workspaces of their own. */
 int64_t pe_attention_paged_workspace_bytes(int64_t M, int batch, int nh, int nkv, int hd, int max_rows,
                                            int64_t max_len, int64_t prefix_len, int dtype);
+int64_t pe_attention_paged_reserve_bytes(int64_t M, int nh, int nkv, int hd, int dtype);
 int pe_tree_attention_paged(const pe_paged_attention_args* args, void* stream);
 
 /* ------------------------------------------------------------ tree proposal */

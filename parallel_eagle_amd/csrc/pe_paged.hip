@@ -74,7 +74,9 @@ __device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* red) {
 // of every gridDim.x-th run of 256 rows and x == 0 its table entries; the last
 // column of blocks (b == batch) marks the rows behind the last sequence.
 // Bound by the launch and a chain of three dependent loads (lengths, free
-// page, slot store): 64 KiB of slots a microsecond and more once rows abound.
+// page, slot store): 3.2 us for eight trees of 26 rows, 4.4 for 256 prompts of
+// 1000 rows on average (2 MB of slots and 66 KB of table entries, 0.4 us at the
+// rate of a copy), the second launch of an update in place included.
 constexpr int kTabThreads = 256;
 
 __global__ __launch_bounds__(kTabThreads) void page_tables_kernel(
@@ -217,7 +219,10 @@ __global__ __launch_bounds__(kTabThreads) void page_release_kernel(const int32_t
 // the piece of V-byte vectors, `vpr` of them, moved by `vpr` neighbouring
 // lanes. Pieces run over the rows of one head first: those are neighbours both
 // in a page and in a contiguous cache, so a wave's stores fill whole KiB of a
-// page. Each thread has its kWriteUnroll loads in flight before the first store.
+// page. Each thread has its kWriteUnroll loads in flight before the first store,
+// the slot's among them. Bound by HBM: 2000 rows of 32 heads of 256 bytes in 8
+// layers, 524 MB read and written, 104 us, the rate of a large copy; 208 rows
+// of 8 heads in one layer take 7.8 us, a launch and two dependent loads.
 constexpr int kWriteUnroll = 4;
 
 template <typename V>
@@ -282,8 +287,10 @@ __global__ __launch_bounds__(256) void slot_offsets_kernel(const int64_t* __rest
 // one run of rows (four of 256 bytes) of kCompactHeads (layer, head) pairs at a
 // time, all loads before the first store. Where the rows lie is worked out once
 // per run, for all those heads: with one pair to a wave those 64-bit products
-// were the kernel's time (18 us for 32 trees of 64 nodes, 8 layers of 32 heads;
-// 33 MB). What is left is the chain length and path, table entries, rows.
+// were the kernel's time (21.8 us for 32 trees of 40 to 64 nodes, 8 layers of 32
+// heads, 33 MB; 14.0 now, 6.8 at the rate of a copy. Eight trees of 26 nodes, 48
+// layers of 8 heads: 18.2 and 6.4, 2.5). What is left is the chain length and
+// path, table entries, rows.
 constexpr int kCompactHeads = 8;
 
 template <typename V>
@@ -360,12 +367,13 @@ __global__ __launch_bounds__(256) void kv_compact_paged_kernel(
 // ---------------------------------------------------------------------------
 // Attention on the VALU
 // ---------------------------------------------------------------------------
-// fp32, and the head sizes that the matrix-core kernel does not take: one block
-// per (row, query head) and part of the row's keys, LPK lanes (four dims each)
-// on one key, 256 / LPK keys in step. Each key slot keeps its own running
-// maximum, sum and weighted V (one pass, any length); the slots are joined in
-// LDS in slot order. Scores, weights and sums are fp32 throughout. Bound by the
-// latency of a slot's loads (kValuKeys keys in flight).
+// fp32, and the head sizes and alignments that the matrix-core kernels do not
+// take: one block per (row, query head), LPK lanes (four dims each) on one key,
+// 256 / LPK keys in step. Each key slot keeps its own running maximum, sum and
+// weighted V (one pass, any length); the slots are joined in LDS in slot order.
+// Scores, weights and sums are fp32 throughout. Bound by the latency of a slot's
+// loads (kValuKeys keys in flight): 5.8 us for two fp32 trees of up to 8 nodes
+// over up to 104 keys, 4 heads of 64.
 constexpr int kValuKeys = 4;
 
 template <int DT, int LPK, bool VEC>

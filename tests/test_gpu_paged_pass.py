@@ -154,6 +154,16 @@ def test_a_server_over_pages(weights, dtype, heads, prefix):
     s.step([12, 12, 12], [1, 1, 1])
 
 
+@pytest.mark.parametrize("weights,dtype", [("nf4", "bfloat16"), ("dense", "float16")])
+def test_prompts_of_more_than_256_rows(weights, dtype):
+    """Chunks of several prompts in one pass of more rows than one row block of the linears."""
+    s = Server(small(weights, dtype), 6, 3, 37)
+    s.append([200, 120, 7])
+    s.append([1, 1, 1])
+    s.append([20, 100, 200])
+    s.step([12, 26, 1], [1, 0, 1])
+
+
 def test_loading_a_prefilled_cache():
     """Rows moved from contiguous caches give the pass the same values: the next pass equals one over the rows that the
     paged cache appended itself, bit for bit."""
