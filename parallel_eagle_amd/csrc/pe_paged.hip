@@ -217,14 +217,12 @@ __global__ __launch_bounds__(kTabThreads) void page_release_kernel(const int32_t
 // ---------------------------------------------------------------------------
 // A copy of rows x nkv pieces of one head's row each (K and V, every layer):
 // the piece of V-byte vectors, `vpr` of them, moved by `vpr` neighbouring
-// lanes. Pieces run over the rows of one head first: those are neighbours both
-// in a page and in a contiguous cache, so a wave's stores fill whole KiB of a
-// page. Each thread has its kWriteUnroll loads in flight before the first store,
-// the slot's among them. Bound by HBM: 2000 rows of 32 heads of 256 bytes in 8
-// layers, 524 MB read and written, 104 us, the rate of a large copy; 208 rows
-// of 8 heads in one layer take 7.8 us, a launch and two dependent loads.
-constexpr int kWriteUnroll = 4;
-
+// lanes, one vector a thread. Pieces run over the rows of one head first: those
+// are neighbours both in a page and in a contiguous cache, so a wave's stores
+// fill whole KiB of a page. A row's slot and its values are asked for together.
+// Bound by HBM: 2000 rows of 32 heads of 256 bytes in 8 layers, 524 MB read and
+// written, 91 us (5.8 TB/s; a large copy reaches 4.97); four vectors a thread: 95.
+// 208 rows of 8 heads in one layer take 2.5 us, a launch and one load's latency.
 template <typename V>
 __global__ __launch_bounds__(256) void kv_write_kernel(
     const uint8_t* __restrict__ ks, const uint8_t* __restrict__ vs, int64_t sl_k, int64_t sr_k, int64_t sh_k,
@@ -236,31 +234,17 @@ __global__ __launch_bounds__(256) void kv_write_kernel(
   const int64_t sr = is_v ? sr_v : sr_k, sh = is_v ? sh_v : sh_k;
   uint8_t* dst = (is_v ? vp : kp) + layer * layer_bytes;
   const uint32_t total = (uint32_t)M * (uint32_t)nkv * (uint32_t)vpr;  // vectors (below 2^31)
-  const uint32_t start = blockIdx.x * (256 * kWriteUnroll) + threadIdx.x;
-  V v[kWriteUnroll];
-  int64_t slot[kWriteUnroll];
-  uint32_t head[kWriteUnroll], col[kWriteUnroll];
-#pragma unroll
-  for (int u = 0; u < kWriteUnroll; ++u) {  // a row's slot and its values are asked for together
-    const uint32_t i = start + u * 256;
-    slot[u] = -1;
-    if (i < total) {
-      const uint32_t piece = i / (uint32_t)vpr;
-      col[u] = i - piece * vpr;
-      head[u] = piece / (uint32_t)M;
-      const uint32_t r = piece - head[u] * M;
-      slot[u] = slots[r];
-      v[u] = *(const V*)(src + r * sr + head[u] * sh + col[u] * sizeof(V));
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < kWriteUnroll; ++u) {
-    if (slot[u] >= 0 && slot[u] < num_slots) {
-      const int64_t page = slot[u] >> ps_log2, at = slot[u] & ((1 << ps_log2) - 1);
-      *(V*)(dst + ((((page * nkv + head[u]) << ps_log2) + at) * vpr + col[u]) * (int64_t)sizeof(V)) = v[u];
-    } else if (slot[u] != -1 && !is_v && layer == 0 && head[u] == 0 && col[u] == 0) {
-      atomicOr(status, PE_ERR_INDEX);
-    }
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const uint32_t piece = i / (uint32_t)vpr, col = i - piece * vpr;
+  const uint32_t head = piece / (uint32_t)M, r = piece - head * M;
+  const int64_t slot = slots[r];
+  const V v = *(const V*)(src + r * sr + head * sh + col * sizeof(V));
+  if (slot >= 0 && slot < num_slots) {
+    const int64_t page = slot >> ps_log2, at = slot & ((1 << ps_log2) - 1);
+    *(V*)(dst + ((((page * nkv + head) << ps_log2) + at) * vpr + col) * (int64_t)sizeof(V)) = v;
+  } else if (slot != -1 && !is_v && layer == 0 && head == 0 && col == 0) {
+    atomicOr(status, PE_ERR_INDEX);
   }
 }
 
@@ -282,25 +266,26 @@ __global__ __launch_bounds__(256) void slot_offsets_kernel(const int64_t* __rest
 // Accepted rows together
 // ---------------------------------------------------------------------------
 // Sequence b's private rows p + path[i] move to p + i, i < len, in every layer
-// and KV head of K and V. path[i] >= i, so a run of rows read whole before the
-// first of them is written never reads what an earlier run wrote: a wave moves
-// one run of rows (four of 256 bytes) of kCompactHeads (layer, head) pairs at a
-// time, all loads before the first store. Where the rows lie is worked out once
-// per run, for all those heads: with one pair to a wave those 64-bit products
-// were the kernel's time (21.8 us for 32 trees of 40 to 64 nodes, 8 layers of 32
-// heads, 33 MB; 14.0 now, 6.8 at the rate of a copy. Eight trees of 26 nodes, 48
-// layers of 8 heads: 18.2 and 6.4, 2.5). What is left is the chain length and
-// path, table entries, rows.
+// and KV head of K and V. path[i] >= i, so rows read before a later one is written
+// hold what they held before the call: a wave (a workgroup of its own) moves one
+// run of rows (four of 256 bytes) of kCompactHeads (layer, head) pairs at a time,
+// all loads before the first store. Where the rows lie is worked out by a lane per
+// row, once for all those pairs, which leaves one chain of length and path, table
+// entries, rows. 32 trees of 40 to 64 nodes, 8 layers of 32 heads (33 MB, partly
+// still in the caches): 6.1 us, 6.2 with 4 pairs to a wave, 6.8 with 16; eight
+// trees of 26 nodes, 48 layers of 8 heads: 3.8. With one pair to a wave each
+// worked the 64-bit places out again, 18 us.
 constexpr int kCompactHeads = 8;
 
 template <typename V>
-__global__ __launch_bounds__(256) void kv_compact_paged_kernel(
+__global__ __launch_bounds__(64) void kv_compact_paged_kernel(
     uint8_t* __restrict__ kp, uint8_t* __restrict__ vp, int64_t layer_bytes, int LH, int nkv, int vpr, int ps_log2,
     const int32_t* __restrict__ table, int64_t ld_table, int64_t cols, int64_t num_pages,
     const int64_t* __restrict__ seq_len, int64_t prefix_len, const int32_t* __restrict__ acc, int64_t ld_acc,
     int max_rows, int32_t* status) {
-  const int b = blockIdx.z;
+  const int b = blockIdx.z, lane = threadIdx.x;
   const int32_t* res = acc + b * ld_acc;
+  int node = res[2 + min(lane, max_rows - 1)];  // asked for beside the length
   const int len = res[0];
   const int64_t p = seq_len[b] - prefix_len;
   const bool first = blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0;
@@ -312,12 +297,21 @@ __global__ __launch_bounds__(256) void kv_compact_paged_kernel(
     if (first) atomicOr(status, len > max_rows ? PE_ERR_INDEX : PE_ERR_CAPACITY);
     return;
   }
-  const int lh0 = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kCompactHeads;
-  if (lh0 >= LH) return;
-  const int lane = threadIdx.x & 63;
+  const int lh0 = blockIdx.x * kCompactHeads;
   uint8_t* pool = blockIdx.y == 0 ? kp : vp;
   const int32_t* tab = table + b * ld_table;
   const int64_t row_bytes = vpr * (int64_t)sizeof(V), head_bytes = row_bytes << ps_log2;
+  int64_t head_at[kCompactHeads];  // of the wave's pairs (the last one again past the end)
+  {
+    int layer = lh0 / nkv, h = lh0 - layer * nkv;
+#pragma unroll
+    for (int k = 0; k < kCompactHeads; ++k) {
+      head_at[k] = layer * layer_bytes + h * head_bytes;
+      const bool more = lh0 + k + 1 < LH, wrap = h + 1 == nkv;
+      layer += more && wrap ? 1 : 0;
+      h = more ? (wrap ? 0 : h + 1) : h;
+    }
+  }
   // byte offset of private row j in KV head 0 of layer 0, -1 where no such row exists
   auto row_at = [&](int64_t j) -> int64_t {
     if (j >= (cols << ps_log2)) return -1;
@@ -329,15 +323,15 @@ __global__ __launch_bounds__(256) void kv_compact_paged_kernel(
   const int per = 64 / lanes;      // rows a load instruction moves
   const int sub = lane / lanes, c0 = lane - sub * lanes;
   bool bad = false;
-  for (int base = 0; base < len; base += per) {
-    const int i = base + sub;
+  for (int i0 = 0; i0 < len; i0 += 64) {
+    const int i = i0 + lane;  // this lane's row
+    if (i0 > 0) node = res[2 + min(i, max_rows - 1)];
     int64_t from = -1, dst = -1;
-    if (sub < per && i < len) {
-      const int n = res[2 + i];
-      if (n < i || n >= max_rows) {
+    if (i < len) {
+      if (node < i || node >= max_rows) {
         bad = true;
-      } else if (n != i) {
-        from = row_at(p + n);
+      } else if (node != i) {
+        from = row_at(p + node);
         dst = row_at(p + i);
         if (from < 0 || dst < 0) {
           bad = true;
@@ -345,19 +339,19 @@ __global__ __launch_bounds__(256) void kv_compact_paged_kernel(
         }
       }
     }
-    for (int c = c0; c < vpr; c += lanes) {
-      V v[kCompactHeads];
+    const int n = min(64, len - i0);
+    for (int r0 = 0; r0 < n; r0 += per) {
+      const int at = r0 + sub;
+      const int64_t rf = __shfl(from, at & 63, 64), rd = __shfl(dst, at & 63, 64);
+      if (sub >= per || at >= n || rd < 0) continue;
+      for (int c = c0; c < vpr; c += lanes) {
+        V v[kCompactHeads];
 #pragma unroll
-      for (int k = 0; k < kCompactHeads; ++k) {
-        const int layer = (lh0 + k) / nkv, h = lh0 + k - layer * nkv;
-        if (lh0 + k < LH && dst >= 0)
-          v[k] = *(const V*)(pool + layer * layer_bytes + h * head_bytes + from + c * (int64_t)sizeof(V));
-      }
+        for (int k = 0; k < kCompactHeads; ++k)  // (past the last pair: its row again)
+          v[k] = *(const V*)(pool + head_at[k] + rf + c * (int64_t)sizeof(V));
 #pragma unroll
-      for (int k = 0; k < kCompactHeads; ++k) {
-        const int layer = (lh0 + k) / nkv, h = lh0 + k - layer * nkv;
-        if (lh0 + k < LH && dst >= 0)
-          *(V*)(pool + layer * layer_bytes + h * head_bytes + dst + c * (int64_t)sizeof(V)) = v[k];
+        for (int k = 0; k < kCompactHeads; ++k)
+          *(V*)(pool + head_at[k] + rd + c * (int64_t)sizeof(V)) = v[k];
       }
     }
   }
@@ -603,14 +597,14 @@ extern "C" int pe_kv_write_paged(const void* k, const void* v, const int64_t* k_
 #define PE_WRITE(V)                                                                                               \
   do {                                                                                                            \
     const int vpr = (int)(row / (int64_t)sizeof(V));                                                              \
-    const int64_t blocks = (M * nkv * vpr + 256 * kWriteUnroll - 1) / (256 * kWriteUnroll);                       \
+    const int64_t blocks = (M * nkv * vpr + 255) / 256;                                                           \
     if (M * nkv * vpr >= (int64_t(1) << 31)) return PE_ERR_ARG;                                                   \
     kv_write_kernel<V><<<dim3((unsigned)blocks, L, 2), 256, 0, st>>>(                                             \
         (const uint8_t*)k, (const uint8_t*)v, k_strides[0] * es, k_strides[1] * es, k_strides[2] * es,            \
         v_strides[0] * es, v_strides[1] * es, v_strides[2] * es, (uint8_t*)k_pool, (uint8_t*)v_pool, layer_bytes, \
         slots, (int)M, nkv, vpr, psl, num_pages * page_size, status);                                             \
   } while (0)
-  if (any % 16 == 0) PE_WRITE(uint4);
+  if (any % 16 == 0) PE_WRITE(u32x4_t);
   else if (any % 4 == 0) PE_WRITE(uint32_t);
   else PE_WRITE(uint16_t);
 #undef PE_WRITE
@@ -631,14 +625,14 @@ extern "C" int pe_kv_compact_paged(void* k_pool, void* v_pool, int L, int nkv, i
   const int64_t row = (int64_t)hd * es;
   const uint64_t any = (uint64_t)(uintptr_t)k_pool | (uint64_t)(uintptr_t)v_pool | (uint64_t)row;
   const int64_t layer_bytes = num_pages * nkv * page_size * row;
-  const dim3 grid(pe_cdiv((int64_t)L * nkv, 4 * kCompactHeads), 2, batch);
+  const dim3 grid(pe_cdiv((int64_t)L * nkv, kCompactHeads), 2, batch);
   hipStream_t st = (hipStream_t)stream;
 #define PE_COMPACT(V)                                                                                             \
-  kv_compact_paged_kernel<V><<<grid, 256, 0, st>>>((uint8_t*)k_pool, (uint8_t*)v_pool, layer_bytes, L * nkv, nkv, \
+  kv_compact_paged_kernel<V><<<grid, 64, 0, st>>>((uint8_t*)k_pool, (uint8_t*)v_pool, layer_bytes, L * nkv, nkv, \
                                                    (int)(row / (int64_t)sizeof(V)), psl, block_table, ld_table,   \
                                                    cols, num_pages, seq_len, prefix_len, accept_out,              \
                                                    2 + (int64_t)max_rows, max_rows, status)
-  if (any % 16 == 0) PE_COMPACT(uint4);
+  if (any % 16 == 0) PE_COMPACT(u32x4_t);
   else if (any % 4 == 0) PE_COMPACT(uint32_t);
   else PE_COMPACT(uint16_t);
 #undef PE_COMPACT
