@@ -10,6 +10,7 @@ stay plain functions. There is no CPU implementation behind any of them.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -413,7 +414,8 @@ def _device_index(t: torch.Tensor) -> int:
 
 def _vec(t: torch.Tensor, dtype: torch.dtype, n: int, dev: int, name: str) -> int:
     """The pointer of a contiguous vector of at least n elements on device ``dev``."""
-    if t.dtype is not dtype or t.get_device() != dev or t.numel() < n or t.dim() != 1 or not t.is_contiguous():
+    if (t.dtype is not dtype or t.get_device() != dev or t.numel() < n
+            or (t.stride() != (1,) and (t.dim() != 1 or not t.is_contiguous()))):
         raise ValueError(f"{name} must be contiguous {dtype} with at least {n} elements, on the device of the call's "
                          "other tensors")
     return t.data_ptr()
@@ -548,6 +550,11 @@ def attention_paged_reserve_bytes(m: int, nh: int, nkv: int, hd: int, dtype: tor
     return int(lib().pe_attention_paged_reserve_bytes(m, nh, nkv, hd, dcode(dtype)))
 
 
+# The fields of _lib.PagedAttentionArgs in order: packing them at once takes half the time of its constructor
+# (0.8 against 1.6 us a call).
+_PAGED_ARGS = struct.Struct("@13Q11q9i2fi")
+
+
 def tree_attention_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
                          seq_row0: torch.Tensor, seq_len: torch.Tensor, scale: float, max_rows: int, max_len: int,
                          status: torch.Tensor, *, mask_mode: int = _lib.PE_MASK_TREE,
@@ -580,8 +587,7 @@ def tree_attention_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     p_row0, p_len = _vec(seq_row0, torch.int32, b + 1, dev, "seq_row0"), _vec(seq_len, torch.int64, b, dev, "seq_len")
     p_tab, ld, cols = _table(block_table, b, dev)
     p_status = _vec(status, torch.int32, 1, dev, "status")
-    p_bits = p_pos = p_slopes = p_pre = None
-    words = n_pre = 0
+    p_bits = p_pos = p_slopes = p_pre = words = n_pre = 0
     if mask_mode == _lib.PE_MASK_TREE:
         if (bits is None or bits.dtype is not torch.int64 or bits.dim() != 2 or bits.shape[0] < m
                 or not bits.is_contiguous() or bits.get_device() != dev):
@@ -605,16 +611,20 @@ def tree_attention_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     if workspace is None:
         need = attention_paged_workspace_bytes(m, b, nh, nkv, hd, max_rows, max_len, prefix_len, dt)
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    p_ws, ws_bytes = None, 0
+    p_ws = ws_bytes = 0
     if workspace is not None:
         if not workspace.is_contiguous() or workspace.get_device() != dev:
             raise ValueError("workspace must be contiguous, on the device of the call's other tensors")
         p_ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    a = _lib.PagedAttentionArgs(
-        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), p_tab, p_pre, p_row0, p_len, p_bits, p_pos,
-        p_slopes, p_ws, p_status, ws_bytes, ld_q if m > 1 else nh * hd, out.stride(0) if m > 1 else nh * hd, ld, cols,
-        pages, n_pre, prefix_len, max_len, window, m, b, max_rows, nh, nkv, hd, ps, dcode(dt), mask_mode, words, scale,
-        softcap, 0)
+    try:
+        packed = _PAGED_ARGS.pack(
+            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), p_tab, p_pre, p_row0, p_len, p_bits, p_pos,
+            p_slopes, p_ws, p_status, ws_bytes, ld_q if m > 1 else nh * hd, out.stride(0) if m > 1 else nh * hd, ld, cols,
+            pages, n_pre, prefix_len, max_len, window, m, b, max_rows, nh, nkv, hd, ps, dcode(dt), mask_mode, words, scale,
+            softcap, 0)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"tree_attention_paged: a count or scale that its field does not hold ({e})") from e
+    a = _lib.PagedAttentionArgs.from_buffer_copy(packed)
     check(_call_on(dev, lib().pe_tree_attention_paged, C.byref(a)), "pe_tree_attention_paged")
     return out
 

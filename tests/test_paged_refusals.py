@@ -3,6 +3,7 @@ launched: the pointers are never read) and what their wrappers raise."""
 
 import ctypes as C
 import random
+import re
 
 import pytest
 import torch
@@ -176,3 +177,13 @@ def test_wrappers_want_device_tensors():
     with pytest.raises(ValueError):
         ops.tree_attention_paged(torch.zeros(1, 1, 64), torch.zeros(1, 1, 16, 64), torch.zeros(1, 1, 16, 64), z.view(1, 2),
                                  z, torch.zeros(1, dtype=torch.int64), 1.0, 1, 1, z)
+
+
+def test_the_packed_arguments_are_the_structs_fields():
+    """Every field a different value, through the wrapper's format and through the struct's constructor."""
+    fields = _lib.PagedAttentionArgs._fields_
+    codes = {C.c_void_p: "Q", C.c_int64: "q", C.c_int32: "i", C.c_float: "f"}
+    runs = re.findall(r"(\d*)([a-zA-Z])", ops._PAGED_ARGS.format)
+    assert "".join(c * int(n or 1) for n, c in runs) == "".join(codes[t] for _, t in fields)
+    want = [float(i) if t is C.c_float else i for i, (_, t) in enumerate(fields, 1)]
+    assert ops._PAGED_ARGS.pack(*want) == bytes(_lib.PagedAttentionArgs(*want))
