@@ -570,6 +570,33 @@ def test_compact_moves_the_accepted_rows(dtype, hd, page):
     assert torch.equal(pools[0], want[0]) and torch.equal(pools[1], want[1]) and int(st.item()) == 0
 
 
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.float16, 36), (torch.float32, 512)])
+@pytest.mark.parametrize("step", [1, 6])
+def test_compact_of_paths_longer_than_a_wave(dtype, hd, step):
+    """Every row moves `step` rows down, onto rows that others are read from; 15 (layer, head) pairs."""
+    L, nkv, page, T = 5, 3, 16, 200
+    gen = torch.Generator().manual_seed(hd + step)
+    n = T - step
+    priv = [7, 0]
+    pages = [-(-(p + T) // page) for p in priv]
+    perm = torch.randperm(sum(pages), generator=gen).int()
+    table = torch.full((2, max(pages)), -1, dtype=torch.int32)
+    table[0, : pages[0]], table[1, : pages[1]] = perm[: pages[0]], perm[pages[0]:]
+    acc = torch.zeros((2, 2 + T), dtype=torch.int32)
+    acc[:, 0] = n
+    acc[:, 2: 2 + n] = torch.arange(step, T, dtype=torch.int32)
+    pools = [torch.randn((L, sum(pages), nkv, page, hd), generator=gen).to(dtype).to(DEV) for _ in range(2)]
+    want = [p.clone() for p in pools]
+    for w, src in zip(want, pools):
+        for b in range(2):
+            for i in range(n):
+                s, d = priv[b] + step + i, priv[b] + i
+                w[:, int(table[b, d // page]), :, d % page] = src[:, int(table[b, s // page]), :, s % page]
+    st = status_word()
+    ops.kv_compact_paged(pools[0], pools[1], table.to(DEV), torch.tensor(priv, device=DEV), acc.to(DEV), st)
+    assert torch.equal(pools[0], want[0]) and torch.equal(pools[1], want[1]) and int(st.item()) == 0
+
+
 def test_compact_flags_paths_and_pages_that_are_none():
     def call(acc, table=((0, 1),), length=4):
         pools = [torch.arange(2 * 2 * 16 * 8, dtype=torch.float32, device=DEV).view(1, 2, 2, 16, 8) for _ in range(2)]
