@@ -366,8 +366,8 @@ __global__ __launch_bounds__(64) void kv_compact_paged_kernel(
 // 256 / LPK keys in step. Each key slot keeps its own running maximum, sum and
 // weighted V (one pass, any length); the slots are joined in LDS in slot order.
 // Scores, weights and sums are fp32 throughout. Bound by the latency of a slot's
-// loads (kValuKeys keys in flight): 5.8 us for two fp32 trees of up to 8 nodes
-// over up to 104 keys, 4 heads of 64.
+// loads (kValuKeys keys in flight): 5.4 us for two fp32 trees of up to 8 nodes
+// over up to 104 keys, 4 heads of 64; eight of 26 nodes over up to 1900: 96.
 constexpr int kValuKeys = 4;
 
 template <int DT, int LPK, bool VEC>
@@ -430,22 +430,18 @@ __global__ __launch_bounds__(256) void attn_paged_valu_kernel(PagedAttn a) {
         }
         if (a.window > 0) see[k] = see[k] && dist < a.window;
       }
-      int64_t at = -1;
-      if (see[k]) {
-        const bool pre = j < a.prefix_len;
-        const int64_t i = pre ? j : j - a.prefix_len;
-        const int page = (pre ? a.prefix_table : a.block_table + b * a.ld_table)[i >> psl];
-        if (page >= 0 && page < a.num_pages)
-          at = ((((int64_t)page * nkv + kvh) << psl) + (i & ((1 << psl) - 1))) * hd;
-        else
-          bad = true;
-      }
-      see[k] = at >= 0;
+      // loads of a key that is not seen go to one that is there, so that none waits behind a branch
+      const int64_t jj = min(j, end - 1);
+      const bool pre = jj < a.prefix_len;
+      const int64_t i = pre ? jj : jj - a.prefix_len;
+      const int page = (pre ? a.prefix_table : a.block_table + b * a.ld_table)[i >> psl];
+      const bool ok = page >= 0 && page < a.num_pages;
+      bad = bad || (see[k] && !ok);
+      see[k] = see[k] && ok;
+      const int64_t at = see[k] ? ((((int64_t)page * nkv + kvh) << psl) + (i & ((1 << psl) - 1))) * hd : 0;
       sc[k] = slope * (float)dist;
-      if (see[k]) {
-        load4((const Te*)a.k_pool + at, kv[k]);
-        load4((const Te*)a.v_pool + at, vv[k]);
-      }
+      load4((const Te*)a.k_pool + at, kv[k]);
+      load4((const Te*)a.v_pool + at, vv[k]);
     }
 #pragma unroll
     for (int k = 0; k < kValuKeys; ++k) {
